@@ -112,6 +112,7 @@ class GroupGeometry:
     entries: List[int] = field(default_factory=list)     # cache entry ids, in order
     value_dim: int = 0                                   # 0: values as wide as keys
     values_in_keys: bool = False                         # no value pool: values lead the key rows
+    codes: bool = False                                  # 8-bit codes with a scale per page and head
 
     @property
     def v_dim(self) -> int:
@@ -198,12 +199,16 @@ class CacheBook:
 
 
 def plan_groups(requests: Sequence[object], max_tokens: int, max_seq_len: int,
-                n_slots: int) -> Tuple[List[GroupGeometry], Dict[int, Tuple[int, int]]]:
+                n_slots: int, codes: bool = False
+                ) -> Tuple[List[GroupGeometry], Dict[int, Tuple[int, int]]]:
     """Group key/value requests by what they need.
 
     Returns the groups and {cache entry id: (group index, index within group)}.
     ``requests[i]`` is the KVRequest of cache entry i, or something else (no
-    keys and values).
+    keys and values).  ``codes``: keys and values are held as 8-bit codes with a scale
+    per page; a window's ring then has one page more, so that the page being
+    filled holds no key that is still seen.  Latent rows stay as they are;
+    a request that cannot be held so is refused.
     """
     from ..parts.base import KVRequest
     groups: List[GroupGeometry] = []
@@ -214,18 +219,23 @@ def plan_groups(requests: Sequence[object], max_tokens: int, max_seq_len: int,
     for entry, r in enumerate(requests):
         if not isinstance(r, KVRequest):
             continue
-        window = r.window if (r.window is not None and round_up(r.window, PAGE) < full_cap) else None
+        in_keys = bool(getattr(r, "values_in_keys", False))
+        coded = codes and not in_keys
+        if coded and not getattr(r, "eight_bit", False):
+            raise CacheError(f"cache entry {entry} (heads of {r.head_dim}) cannot be held in 8 bits")
+        ring = None if r.window is None else round_up(r.window, PAGE) + (PAGE if coded else 0)
+        window = r.window if ring is not None and ring < full_cap else None
         value_dim = getattr(r, "value_dim", 0)
         if value_dim == r.head_dim:
             value_dim = 0
-        in_keys = bool(getattr(r, "values_in_keys", False))
         key = (r.n_kv_heads, r.head_dim, window, value_dim, in_keys)
         if key not in index:
-            cap = full_cap if window is None else round_up(window, PAGE)
+            cap = full_cap if window is None else ring
             n_pages = min(budget_pages, n_slots * (cap // PAGE))
             index[key] = len(groups)
             groups.append(GroupGeometry(r.n_kv_heads, r.head_dim, window, cap, max(1, n_pages),
-                                        value_dim=value_dim, values_in_keys=in_keys))
+                                        value_dim=value_dim, values_in_keys=in_keys,
+                                        codes=coded))
         g = index[key]
         where[entry] = (g, len(groups[g].entries))
         groups[g].entries.append(entry)

@@ -8,6 +8,12 @@ rows (a latent that serves as both) has the one pool.  Position p of the sequenc
 row p % cap; its page is ``page_table[s, row // PAGE]``.  Nothing is cleared
 when a slot is reused: every read is bounded by the sequence's length.
 
+With ``kv_dtype`` torch.float8_e4m3fn the groups whose mixers can work from 8-bit codes hold those,
+and beside each pool one 32-bit power-of-two scale for each page and kv head: a value is code *
+scale.  A window's ring then has a page more than the window takes, so that the page being filled
+never holds keys that are still seen and its scale is that of its own tokens alone.  Latent
+groups (values that lead the key rows) stay in the compute dtype.
+
 Fixed-size state is ``[entries, slots, numel]`` in 32-bit and is zeroed when a
 slot is acquired.
 """
@@ -31,6 +37,8 @@ class KVView:
     page: int
     cap: int
     window: Optional[int]
+    k_scale: Optional[torch.Tensor] = None    # [pages, nkv] float32 of an entry held as codes
+    v_scale: Optional[torch.Tensor] = None
 
 
 @dataclass
@@ -40,7 +48,8 @@ class StateView:
 
 class Cache:
     def __init__(self, requests: Sequence[object], max_tokens: int, max_seq_len: int,
-                 n_slots: int, dtype: torch.dtype, device: torch.device):
+                 n_slots: int, dtype: torch.dtype, device: torch.device,
+                 kv_dtype: Optional[torch.dtype] = None):
         # an entry asks for keys and values, for fixed-size state, for both (a tuple of the
         # two requests) or for nothing
         self.requests = list(requests)
@@ -56,18 +65,32 @@ class Cache:
         max_seq_len = max(1, min(max_seq_len, round_up(max_tokens, PAGE)))
         self.max_seq_len = max_seq_len
         self.max_tokens = max_tokens
-        groups, self.where = plan_groups(kv_requests, max_tokens, max_seq_len, n_slots)
+        if kv_dtype not in (None, dtype, torch.float8_e4m3fn):
+            raise CacheError(f"the cache holds the compute dtype ({dtype}) or float8_e4m3fn, not "
+                             f"{kv_dtype}")
+        groups, self.where = plan_groups(kv_requests, max_tokens, max_seq_len, n_slots,
+                                         codes=kv_dtype == torch.float8_e4m3fn)
+        if kv_dtype == torch.float8_e4m3fn and not any(g.codes for g in groups):
+            raise CacheError("no layer of this model holds keys and values that 8-bit codes can stand "
+                             "for")
         self.book = CacheBook(groups, n_slots, max_seq_len)
         self.n_slots = n_slots
         self.k_pools: List[torch.Tensor] = []
         self.v_pools: List[torch.Tensor] = []
         self.tables: List[torch.Tensor] = []
+        self.scales: List[Optional[torch.Tensor]] = []     # [2, entries, pages, nkv], or None
         for g in groups:
             shape = (len(g.entries), g.n_pages, PAGE, g.n_kv_heads)
-            self.k_pools.append(torch.zeros(shape + (g.head_dim,), dtype=dtype, device=device))
+
+            def pool(dim):
+                if not g.codes:
+                    return torch.zeros(shape + (dim,), dtype=dtype, device=device)
+                return torch.zeros(shape + (dim,), dtype=torch.uint8, device=device).view(kv_dtype)
+            self.k_pools.append(pool(g.head_dim))
             # (a group whose values lead its key rows has one pool under both names)
-            self.v_pools.append(self.k_pools[-1] if g.values_in_keys else
-                                torch.zeros(shape + (g.v_dim,), dtype=dtype, device=device))
+            self.v_pools.append(self.k_pools[-1] if g.values_in_keys else pool(g.v_dim))
+            self.scales.append(torch.ones((2, len(g.entries), g.n_pages, g.n_kv_heads),
+                                          dtype=torch.float32, device=device) if g.codes else None)
             self.tables.append(torch.zeros((n_slots, g.max_pages), dtype=torch.int32,
                                            device=device))
         # fixed-size state: one tensor per distinct size
@@ -128,8 +151,9 @@ class Cache:
             raise CacheError(f"cache entry {entry} holds no keys and values")
         gi, li = self.where[entry]
         g = self.book.groups[gi]
+        sc = self.scales[gi]
         return KVView(self.k_pools[gi][li], self.v_pools[gi][li], self.tables[gi], PAGE, g.cap,
-                      g.window)
+                      g.window, *((sc[0, li], sc[1, li]) if sc is not None else ()))
 
     def state_view(self, entry: int) -> StateView:
         if entry not in self.state_where:
@@ -140,7 +164,8 @@ class Cache:
     def bytes_held(self) -> int:
         n = 0
         seen = set()
-        for t in self.k_pools + self.v_pools + self.states + self.tables:
+        scales = [s for s in self.scales if s is not None]
+        for t in self.k_pools + self.v_pools + self.states + self.tables + scales:
             if t.data_ptr() in seen:
                 continue
             seen.add(t.data_ptr())

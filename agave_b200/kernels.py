@@ -55,6 +55,7 @@ def library() -> ctypes.CDLL:
                     raise KernelError(f"the CUDA library {path} could not be loaded: {e}") from None
                 lib.agv_last_error.restype = ctypes.c_char_p
                 lib.agv_attention_prefill_tc_vt_cols.restype = ctypes.c_longlong
+                lib.agv_attention_decode_e4m3_scratch.restype = ctypes.c_longlong
                 if os.environ.get("AGAVE_B200_DEPENDENT_LAUNCH", "1") == "0":
                     # kernels then start only after the one before has ended, which
                     # makes per-kernel durations in a profiler additive
@@ -133,6 +134,20 @@ def _i32(t: Optional[torch.Tensor], what: str) -> None:
 def _f32(t: Optional[torch.Tensor], what: str) -> None:
     if t is not None and t.dtype != torch.float32:
         raise KernelError(f"{what} must be float32, got {t.dtype}")
+
+
+def _require(ok: bool, message: str) -> None:
+    if not ok:
+        raise KernelError(message)
+
+
+def _on_current_device(*tensors) -> None:
+    """All given tensors lie on the CUDA device that is current: the launch goes to its stream."""
+    dev = _raw_device() if _raw_device is not None else torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and not (t.is_cuda and t.get_device() == dev):
+            raise KernelError(f"a tensor on {t.device} was handed to a kernel; the current CUDA "
+                              f"device is cuda:{dev}")
 
 
 def device_arch() -> int:
@@ -1802,9 +1817,10 @@ def attention_prefill(q, k, v, out, ctx, n_heads, n_kv_heads, head_dim, scale, w
                                    softcap=softcap)
 
 
-def _attention_cost(ctx, q, k, v, out, n_heads, head_dim, window, n_kv_heads=0):
+def _attention_cost(ctx, q, k, v, out, n_heads, head_dim, window, n_kv_heads=0, cache_bytes=0):
     """(bytes, flops) of one layer's attention, from the lengths the host knows
-    (``ctx.lens_host``; zeros when a step does not carry them)."""
+    (``ctx.lens_host``; zeros when a step does not carry them).  ``cache_bytes``: of an element
+    of the cache where that is not the output's type."""
     if _perf is None:
         return 0, 0
     lens = getattr(ctx, "lens_host", None)
@@ -1825,7 +1841,7 @@ def _attention_cost(ctx, q, k, v, out, n_heads, head_dim, window, n_kv_heads=0):
             seen += window * (window + 1) // 2 + (n - window) * window
         else:
             seen += n * (n + 1) // 2
-    esz = out.element_size()
+    esz = cache_bytes or out.element_size()
     nbytes = _nbytes(q, k, v, out) + 2 * kv_rows * n_kv_heads * head_dim * esz
     return nbytes, 4 * n_heads * head_dim * seen
 
@@ -1972,7 +1988,14 @@ def attention_decode(q, out, view, ctx, n_heads, n_kv_heads, head_dim, scale, wi
                      values_in_keys: bool = False, op: str = "attention",
                      keep_first: int = 0, softcap: float = 0.0) -> None:
     """Decode attention of one layer: the split kernel for key and value head sizes in steps
-    of 16 up to 512, else the one-warp-per-head kernel."""
+    of 16 up to 512, else the one-warp-per-head kernel; a cache entry that holds 8-bit codes
+    goes to ``attention_decode_e4m3``."""
+    if getattr(view, "k_scale", None) is not None:
+        _require(not values_in_keys, "values that are part of the key rows are not held in 8 bits")
+        attention_decode_e4m3(q, out, view, ctx, n_heads, n_kv_heads, head_dim, scale, window,
+                              value_dim=value_dim, sinks=sinks, dist_bias=dist_bias,
+                              keep_first=keep_first, softcap=softcap, op=op)
+        return
     hdv = value_dim or head_dim
     if not window:
         keep_first = 0
@@ -1995,3 +2018,160 @@ def attention_decode(q, out, view, ctx, n_heads, n_kv_heads, head_dim, scale, wi
                                  dist_bias=dist_bias,
                                  v_row=n_kv_heads * head_dim if values_in_keys else 0,
                                  keep_first=keep_first, softcap=softcap)
+
+
+# --------------------------------------------------------------- the 8-bit cache
+E4M3 = torch.float8_e4m3fn
+E4M3_MAX_HEAD = 256
+
+
+def e4m3_head_supported(head_dim: int, value_dim: int = 0) -> bool:
+    """Whether keys and values of these head sizes can be held and attended as e4m3 codes."""
+    return all(d % 16 == 0 and 0 < d <= E4M3_MAX_HEAD for d in (head_dim, value_dim or head_dim))
+
+
+def _e4m3_view(view, n_kv_heads: int, head_dim: int, value_dim: int, what: str):
+    """Checks a cache entry's pools, scales and table; (slots of the table, its width, pages)."""
+    k, v, table = view.k_pool, view.v_pool, view.page_table
+    _require(k.dtype == E4M3 and v.dtype == E4M3, f"{what}: the pools must hold float8_e4m3fn codes")
+    _require(k.dim() == 4 and v.dim() == 4 and k.shape[1:] == (view.page, n_kv_heads, head_dim) and
+             v.shape[1:] == (view.page, n_kv_heads, value_dim) and v.shape[0] == k.shape[0],
+             f"{what}: pools {tuple(k.shape)} and {tuple(v.shape)} are not [pages, {view.page}, "
+             f"{n_kv_heads}, head size]")
+    _require(k.is_contiguous() and v.is_contiguous() and table.is_contiguous() and
+             view.k_scale.is_contiguous() and view.v_scale.is_contiguous(),
+             f"{what}: pools, scales and page table must be contiguous")
+    for s in (view.k_scale, view.v_scale):
+        _require(s.dtype == torch.float32 and s.shape == (k.shape[0], n_kv_heads),
+                 f"{what}: scales must be float32 [{k.shape[0]}, {n_kv_heads}]")
+    _i32(table, "page_table")
+    return table.shape[0], table.shape[1], k.shape[0]
+
+
+def cache_store_e4m3(k: torch.Tensor, v: torch.Tensor, view, ctx, n_kv_heads: int, head_dim: int,
+                     value_dim: int = 0) -> None:
+    """Stores the step's keys k [T, nkv * hd] and values v [T, nkv * hdv] (rows may be strided)
+    in the cache entry ``view``, whose pools hold e4m3 codes [pages, page, nkv, size] and whose
+    ``k_scale``, ``v_scale`` hold one 32-bit power of two for each page and head.
+
+    ctx: ``cu_seqlens`` [B + 1], ``slots`` and ``lens`` [B] (the length after the step), and
+    ``max_new``, the most tokens an entry brings.  The scale is the smallest 2^e (e >= -126)
+    with 448 * 2^e >= every finite magnitude of the page and head; a page that already holds
+    tokens of its sequence keeps its scale or, where a new token needs a greater one, has their
+    codes rounded to that.  Values that are not finite are held as NaN.  Where ``cap`` wraps
+    around (a window's ring), it must leave a page more than the window takes.  A slot may
+    appear once; entries with a negative slot store nothing."""
+    hdv = value_dim or head_dim
+    _on_current_device(k, v, view.k_pool, view.v_pool, view.k_scale, view.v_scale, view.page_table,
+                       ctx.cu_seqlens, ctx.slots, ctx.lens)
+    T = k.shape[0]
+    _require(k.dim() == 2 and v.dim() == 2 and k.shape[1] == n_kv_heads * head_dim and
+             v.shape == (T, n_kv_heads * hdv),
+             f"cache_store_e4m3: keys {tuple(k.shape)} and values {tuple(v.shape)} do not fit "
+             f"{n_kv_heads} heads of {head_dim} and {hdv}")
+    _require(k.dtype == v.dtype, f"cache_store_e4m3: keys {k.dtype} and values {v.dtype} differ")
+    _require(k.stride(1) == 1 and v.stride(1) == 1, "cache_store_e4m3: elements of a row must be adjacent")
+    n_slots, max_pages, n_pages = _e4m3_view(view, n_kv_heads, head_dim, hdv, "cache_store_e4m3")
+    cu, slots, lens = ctx.cu_seqlens, ctx.slots, ctx.lens
+    _i32(cu, "cu_seqlens"); _i32(slots, "slots"); _i32(lens, "lens")
+    B = slots.numel()
+    _require(cu.numel() == B + 1 and lens.numel() == B and cu.is_contiguous() and
+             slots.is_contiguous() and lens.is_contiguous(),
+             "cache_store_e4m3: cu_seqlens [B + 1], slots [B] and lens [B] do not fit")
+    with _span("cache_store", T * n_kv_heads * (head_dim + hdv) * (k.element_size() + 1)):
+        _check(library().agv_cache_store_e4m3(
+            _ptr(k), ctypes.c_longlong(k.stride(0)), _ptr(v), ctypes.c_longlong(v.stride(0)),
+            dtype_code(k.dtype), _ptr(cu), _ptr(slots), _ptr(lens), B, T, int(ctx.max_new),
+            n_kv_heads, head_dim, hdv, _ptr(view.k_pool), _ptr(view.v_pool), _ptr(view.k_scale),
+            _ptr(view.v_scale), _ptr(view.page_table), n_slots, max_pages, view.page, view.cap,
+            n_pages, _stream()))
+
+
+def attention_decode_e4m3(q: torch.Tensor, out: torch.Tensor, view, ctx, n_heads: int,
+                          n_kv_heads: int, head_dim: int, scale: float, window: int,
+                          value_dim: int = 0, sinks: Optional[torch.Tensor] = None,
+                          dist_bias: Optional[torch.Tensor] = None, keep_first: int = 0,
+                          softcap: float = 0.0, op: str = "attention") -> None:
+    """Decode attention of one layer over a cache entry that holds e4m3 codes
+    (``cache_store_e4m3``): q [B, nh * hd] (rows may be strided) at ``ctx.positions``, out
+    [B, nh * hdv] of the same type.  Codes are exact in the products; sums, the softmax and its
+    weights are 32-bit (of bfloat16 queries the weights are rounded to 11 bits).  Options as in
+    ``attention_decode``; rows of entries with a negative slot become zeros.  ``ctx.max_len``
+    bounds the lengths (it sizes the grid and the scratch; a longer sequence is still walked
+    whole)."""
+    hdv = value_dim or head_dim
+    slots, positions = ctx.slots, ctx.positions
+    _require(e4m3_head_supported(head_dim, hdv),
+             f"attention_decode_e4m3: head sizes {head_dim} and {hdv} must be multiples of 16 up to "
+             f"{E4M3_MAX_HEAD}")
+    _on_current_device(q, out, view.k_pool, view.v_pool, view.k_scale, view.v_scale,
+                       view.page_table, slots, positions, sinks, dist_bias)
+    B = q.shape[0]
+    _require(q.dim() == 2 and q.shape[1] == n_heads * head_dim and q.stride(1) == 1,
+             f"attention_decode_e4m3: queries {tuple(q.shape)} are not [B, {n_heads} * {head_dim}]")
+    _require(out.dtype == q.dtype and out.is_contiguous() and out.shape == (B, n_heads * hdv),
+             f"attention_decode_e4m3: the output must be contiguous [{B}, {n_heads * hdv}] of {q.dtype}")
+    n_slots, max_pages, n_pages = _e4m3_view(view, n_kv_heads, head_dim, hdv, "attention_decode_e4m3")
+    _i32(slots, "slots"); _i32(positions, "positions"); _f32(sinks, "sinks"); _f32(dist_bias, "dist_bias")
+    _require(slots.numel() == B and positions.numel() == B and slots.is_contiguous() and
+             positions.is_contiguous(), "attention_decode_e4m3: one slot and position per query")
+    _require(sinks is None or (sinks.numel() == n_heads and sinks.is_contiguous()),
+             "attention_decode_e4m3: one sink per query head")
+    _require(dist_bias is None or (dist_bias.dim() == 2 and dist_bias.shape[0] == n_heads and
+                                   dist_bias.is_contiguous()),
+             "attention_decode_e4m3: the bias by distance is [heads, distances]")
+    max_keys = max(1, min(abs(window) + keep_first, ctx.max_len) if window else ctx.max_len)
+    lib = library()
+    floats = lib.agv_attention_decode_e4m3_scratch(B, n_heads, n_kv_heads, head_dim, hdv, max_keys)
+    if floats < 0:
+        _check(floats)
+    partial = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
+    with _span(op, *_attention_cost(ctx, q, None, None, out, n_heads, head_dim, window, n_kv_heads,
+                                    1)):
+        _check(lib.agv_attention_decode_e4m3(
+            _ptr(q), ctypes.c_longlong(q.stride(0)), _ptr(out), dtype_code(q.dtype),
+            _ptr(view.k_pool), _ptr(view.v_pool), _ptr(view.k_scale), _ptr(view.v_scale),
+            _ptr(view.page_table), n_slots, max_pages, view.page, view.cap, n_pages, _ptr(slots),
+            _ptr(positions), B, n_heads, n_kv_heads, head_dim, hdv, ctypes.c_float(scale), window,
+            int(keep_first), _ptr(sinks), _ptr(dist_bias),
+            dist_bias.shape[1] if dist_bias is not None else 0, ctypes.c_float(softcap), max_keys,
+            _ptr(partial), ctypes.c_longlong(floats), _stream()))
+
+
+# ------------------------------------------------------------- log-probabilities
+LOGPROBS_MAX_TOP = 32
+
+
+class TokenLogprobs:
+    """What ``token_logprobs`` finds for R rows: ``logprob`` and ``entropy`` [R] (32-bit, nats),
+    ``rank`` [R] (int32; 1 = the greatest logit), ``top_ids`` [R, top] (int32) and
+    ``top_logprobs`` [R, top] (32-bit), greatest first, equal ones by index."""
+    __slots__ = ("logprob", "entropy", "rank", "top_ids", "top_logprobs")
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
+    """ln softmax(logits[r])[tokens[r]] for every row of logits [R, V] (32-bit or bfloat16, rows
+    may be strided), the row's entropy, the token's rank and the ``top`` (at most 32) greatest,
+    from one pass over the logits.  A logit of -inf is a probability of zero.  A token outside
+    the vocabulary stands for none: logprob NaN, rank 0.  Rows that have no softmax (NaN or +inf
+    in them, or nothing but -inf) give NaN; NaN stands below every number among the greatest."""
+    _on_current_device(logits, tokens)
+    _require(logits.dim() == 2 and logits.stride(1) == 1, "token_logprobs: logits must be [rows, vocabulary]")
+    R, V = logits.shape
+    _i32(tokens, "tokens")
+    _require(tokens.numel() == R and tokens.is_contiguous(), f"token_logprobs: one token for each of {R} rows")
+    _require(0 <= top <= min(V, LOGPROBS_MAX_TOP),
+             f"token_logprobs: top {top} must lie in 0..{min(V, LOGPROBS_MAX_TOP)}")
+    r = TokenLogprobs()
+    # one allocation: three columns of R, two of R * top
+    floats = torch.empty((3 + 2 * top) * R, dtype=torch.float32, device=logits.device)
+    ints = floats.view(torch.int32)
+    r.logprob, r.entropy, r.rank = floats[:R], floats[R:2 * R], ints[2 * R:3 * R]
+    r.top_ids = ints[3 * R:(3 + top) * R].view(R, top)
+    r.top_logprobs = floats[(3 + top) * R:].view(R, top)
+    with _span("token_logprobs", _nbytes(logits, floats)):
+        _check(library().agv_token_logprobs(
+            _ptr(logits), ctypes.c_longlong(logits.stride(0)), dtype_code(logits.dtype), R, V,
+            _ptr(tokens), top, _ptr(r.logprob), _ptr(r.entropy), _ptr(r.rank), _ptr(r.top_ids),
+            _ptr(r.top_logprobs), _stream()))
+    return r

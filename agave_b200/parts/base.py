@@ -21,7 +21,7 @@ is all that a new part needs.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Callable, Dict, Optional, Tuple
 
 
@@ -49,12 +49,14 @@ class KVRequest:
     the last W.  ``value_dim``: the size of a value head where it differs from the
     keys' ``head_dim`` (0: the same).  ``values_in_keys``: a position's value is the leading
     ``value_dim`` elements of its key row, so the group holds one pool, not two (a latent that
-    serves as key and as value)."""
+    serves as key and as value).  ``eight_bit``: the mixer can also work from a cache that
+    holds e4m3 codes with a scale per page and head."""
     n_kv_heads: int
     head_dim: int
     window: Optional[int] = None
     value_dim: int = 0
     values_in_keys: bool = False
+    eight_bit: bool = field(default=False, compare=False)
 
 
 @dataclass(frozen=True)
