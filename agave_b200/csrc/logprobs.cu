@@ -1,41 +1,87 @@
 // Log-probabilities of given tokens from rows of logits: ln softmax at the token, the row's
 // entropy, the token's rank and the greatest logits with their indices.
 //
-// With m the row's maximum, s = sum e^(x - m) and t = sum (x - m) e^(x - m): ln p = x_t - m -
-// ln s, H = ln s - t / s.  The greatest are found as 64-bit keys (value, lower index first).
+// With a reference c, d = x - c, s = sum e^d and t = sum d e^d: ln p = x_t - c - ln s and H = ln s -
+// t / s.  Every thread's reference is the greatest logit it has seen; sums move to another
+// reference c' as s' = s e^(c - c'), t' = (t + (c - c') s) e^(c - c').  (x - c comes before the factor
+// log2 e of the exponential: logits may be the type's lowest value.)
+//
+// What bounds it is reading the logits once.  A row is the work of a cluster of 1 to 16 CTAs; a
+// thread takes every LP_THREADS-th 16 bytes of its CTA's slice, four of them under way, and keeps a
+// running maximum, the two sums and the count of logits ahead of the token's.
+//
+// The greatest: a logit and its index are one 64-bit key.  Every thread knows the greatest key
+// it has seen (the running maximum tells it when to look), so the top-th greatest of the threads' keys
+// is a bound that at least ``top`` keys of the slice reach, and beside those threads' own keys hardly
+// any other does.  The slices of the few threads that reach it are read once more (from
+// L2) and ranked; the cluster's first CTA merges the slices' lists.
 #include "common.cuh"
 
 namespace {
 
 constexpr int LP_THREADS = 512;
+constexpr int LP_WARPS = LP_THREADS / 32;
 constexpr int LP_MAX_TOP = 32;
+constexpr int LP_MAX_CLUSTER = 16;
+constexpr int LP_LIST = 2048;             // keys at or above the bound that a CTA can list
+constexpr float LOG2E = 1.4426950408889634f;
+
+typedef unsigned long long u64;
 
 // A logit and its index as one unsigned number that grows with the logit and falls with the
-// index: equal logits (-0 is 0) go by the lower index.  NaN stands below every number.
-__device__ __forceinline__ unsigned long long lp_key(float x, unsigned i) {
+// index: equal logits (-0 is 0) go by the lower index.  NaN stands below every number; no key is 0.
+__device__ __forceinline__ u64 lp_key(float x, unsigned i) {
     unsigned b = __float_as_uint(x + 0.f);
     b = (int)b < 0 ? ~b : b | 0x80000000u;
     if (x != x) b = 0;
-    return (unsigned long long)b << 32 | (0xffffffffu - i);
+    return (u64)b << 32 | (0xffffffffu - i);
 }
-__device__ __forceinline__ float lp_value(unsigned long long key) {
+__device__ __forceinline__ float lp_value(u64 key) {
     const unsigned b = (unsigned)(key >> 32);
     if (b == 0) return __uint_as_float(0x7fffffffu);
     return __uint_as_float((b & 0x80000000u) ? b & 0x7fffffffu : ~b);
 }
-__device__ __forceinline__ unsigned long long warp_max_u64(unsigned long long v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const unsigned long long t = __shfl_xor_sync(0xffffffffu, v, o);
-        v = t > v ? t : v;
-    }
-    return v;
+__device__ __forceinline__ u64 greater(u64 a, u64 b) { return a > b ? a : b; }
+
+__device__ __forceinline__ float lp_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {        // NaN if either is
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
+// s and t relative to the reference c (-inf: nothing yet).
+struct Sums {
+    float c, s, t;
+    __device__ __forceinline__ void move(float to) {
+        // (a reference of -inf has sums of 0, or NaN, which stay that)
+        const float d = fmaxf(c - to, -1e4f), f = lp_ex2(d * LOG2E);
+        t = f * fmaf(d, s, t);
+        s *= f;
+        c = to;
+    }
+    __device__ __forceinline__ void join(float oc, float os, float ot) {
+        Sums o{oc, os, ot};
+        const float to = fmaxf(c, o.c);
+        if (to == -INFINITY) {                    // (only NaN may be in them)
+            s += o.s;
+            return;
+        }
+        move(to);
+        o.move(to);
+        s += o.s;
+        t += o.t;
+    }
+};
 
 struct Logprobs {
     const void* logits;
     long long ld;
-    int V, top;
+    int V, top, cluster;
     const int* tokens;
     float *logprob, *entropy;
     int* rank;
@@ -43,53 +89,345 @@ struct Logprobs {
     float* top_logprobs;
 };
 
-template <typename T>
-__global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(Logprobs a) {
+// What the CTAs of a cluster hand to its first one.
+struct Slice {
+    float c, s, t;
+    int ahead;
+    u64 keys[LP_MAX_TOP];
+};
+
+__device__ __forceinline__ unsigned lp_cluster_rank() {
+    unsigned r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void lp_cluster_arrive() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void lp_cluster_wait() {
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ unsigned in_first_cta(const void* mine) {
+    unsigned p;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(p) : "r"((unsigned)__cvta_generic_to_shared(mine)));
+    return p;
+}
+__device__ __forceinline__ void put(unsigned at, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
+}
+__device__ __forceinline__ void put(unsigned at, int v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
+__device__ __forceinline__ void put(unsigned at, u64 v) {
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory");
+}
+
+// 16 bytes of logits
+template <typename T> struct Piece;
+template <> struct Piece<float> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ void load(const float* p, float* x) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(p));
+        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    }
+};
+template <> struct Piece<__nv_bfloat16> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void load(const __nv_bfloat16* p, float* x) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+        const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+};
+
+// The 32 keys of a warp's lanes, greatest first (a bitonic sort).
+__device__ __forceinline__ u64 sorted(u64 k, int lane) {
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int o = size >> 1; o > 0; o >>= 1) {
+            const u64 p = __shfl_xor_sync(0xffffffffu, k, o);
+            const bool up = (lane & o) == 0, down = (lane & size) == 0 || size == 32;
+            k = (up == down) == (p > k) ? p : k;
+        }
+    return k;
+}
+// The same for keys that rise and then fall (or the other way round).
+__device__ __forceinline__ u64 sorted_bitonic(u64 k, int lane) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const u64 p = __shfl_xor_sync(0xffffffffu, k, o);
+        k = ((lane & o) == 0) == (p > k) ? p : k;
+    }
+    return k;
+}
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(LP_THREADS, 2) logprobs_kernel(const Logprobs a) {
+    constexpr int N = Piece<T>::N, BATCH = 16 / N;         // 16 logits under way, and 64 or 32 bytes
+    __shared__ Sums wsum[LP_WARPS];
+    __shared__ int wahead[LP_WARPS];
+    __shared__ Slice slices[LP_MAX_CLUSTER];               // the first CTA's count
+    __shared__ u64 merge[TOP ? LP_WARPS : 1][32];
+    __shared__ u64 list[TOP ? LP_LIST : 1];
+    __shared__ int n_list;
+    __shared__ u64 bound_key;
+    const int C = a.cluster;
+    if (C > 1) lp_cluster_arrive();                        // (a CTA's memory is written to once it runs)
     pdl_wait();
     pdl_launch_next();
-    __shared__ float scratch[32];
-    __shared__ unsigned long long best[32];
-    const int row = blockIdx.x, tid = threadIdx.x;
+    const int row = blockIdx.x / C, rank = C > 1 ? (int)lp_cluster_rank() : 0;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const T* x = (const T*)a.logits + (long long)row * a.ld;
-    const int t = a.tokens[row];
-    const bool has = t >= 0 && t < a.V;
-    const float xt = has ? to_f32(x[t]) : 0.f;
+    const int tok = a.tokens[row];
+    const bool has = tok >= 0 && tok < a.V;
+    const float xt = has ? to_f32(x[tok]) : INFINITY;
+    // the row as 16-byte pieces behind a head that ends at a 16-byte boundary
+    const int head = min(a.V, (int)((16 - (uintptr_t)x % 16) % 16 / sizeof(T)));
+    const int pieces = (a.V - head) / N, per = (pieces + C - 1) / C;
+    const int v0 = min(pieces, rank * per), v1 = min(pieces, v0 + per);
+
+    Sums sum{-INFINITY, 0.f, 0.f};
     float m = -INFINITY;
-    for (int i = tid; i < a.V; i += LP_THREADS) m = fmaxf(m, to_f32(x[i]));
-    m = block_max(m, scratch);
-    float s = 0.f, w = 0.f, ahead = 0.f;
-    for (int i = tid; i < a.V; i += LP_THREADS) {
-        const float v = to_f32(x[i]), d = v - m, e = expf(d);
-        s += e;
-        if (e > 0.f) w += e * d;
-        ahead += v > xt || (v == xt && i < t);
+    u64 best = 0;
+    int ahead = 0;
+    // x[0 .. n) of indices i, i + 1, ... (in pieces of N, LP_THREADS pieces apart)
+    auto take = [&](const float* v, auto n_const, int i) {
+        constexpr int n = decltype(n_const)::value;
+        float bm = v[0];
+#pragma unroll
+        for (int e = 1; e < n; ++e) bm = fmaxf(bm, v[e]);
+        if (bm > m || (TOP && best == 0)) {
+            if (TOP) {
+#pragma unroll
+                for (int e = 0; e < n; ++e)
+                    best = greater(best, lp_key(v[e], i + e / N * (LP_THREADS * N) + e % N));
+            }
+            if (bm > m) {
+                m = bm;
+                sum.move(m);
+            }
+        }
+        const float c = sum.c == -INFINITY ? 0.f : sum.c;
+#pragma unroll
+        for (int e = 0; e < n; ++e) {
+            // (at e^-150 a term is 0 and its product with d is, too)
+            const float d = max_nan(v[e] - c, -150.f), p = lp_ex2(d * LOG2E);
+            sum.s += p;
+            sum.t = fmaf(p, d, sum.t);
+        }
+        if (bm >= xt) {
+#pragma unroll
+            for (int e = 0; e < n; ++e) {
+                const int at = i + e / N * (LP_THREADS * N) + e % N;
+                ahead += v[e] > xt || (v[e] == xt && at < tok);
+            }
+        }
+    };
+    const T* body = x + head;
+    int v = v0 + tid;
+    for (; v + (BATCH - 1) * LP_THREADS < v1; v += BATCH * LP_THREADS) {
+        float w[BATCH * N];
+#pragma unroll
+        for (int q = 0; q < BATCH; ++q) Piece<T>::load(body + (size_t)(v + q * LP_THREADS) * N, w + q * N);
+        take(w, std::integral_constant<int, BATCH * N>{}, head + v * N);
     }
-    s = block_sum(s, scratch);
-    w = block_sum(w, scratch);
-    ahead = block_sum(ahead, scratch);
-    const float ls = logf(s);
+    for (; v < v1; v += LP_THREADS) {
+        float w[N];
+        Piece<T>::load(body + (size_t)v * N, w);
+        take(w, std::integral_constant<int, N>{}, head + v * N);
+    }
+    // the head and what is left behind the last piece: a thread of the first CTA each
+    const int tail = a.V - head - pieces * N;
+    int edge = -1;
+    if (rank == 0 && tid < head + tail) edge = tid < head ? tid : a.V - tail + tid - head;
+    float xe = 0.f;
+    if (edge >= 0) {
+        xe = to_f32(x[edge]);
+        take(&xe, std::integral_constant<int, 1>{}, edge);
+    }
+    // ---- sums and counts of the CTA
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const float oc = __shfl_xor_sync(0xffffffffu, sum.c, o), os = __shfl_xor_sync(0xffffffffu, sum.s, o);
+        const float ot = __shfl_xor_sync(0xffffffffu, sum.t, o);
+        sum.join(oc, os, ot);
+    }
+    ahead = __reduce_add_sync(0xffffffffu, ahead);
+    if (lane == 0) {
+        wsum[warp] = sum;
+        wahead[warp] = ahead;
+    }
+    if (tid == 0) n_list = 0;
+    u64 k = 0;
+    if (TOP) {
+        k = sorted(best, lane);
+        merge[warp][lane] = k;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        Sums all = wsum[lane & (LP_WARPS - 1)];
+        int n = wahead[lane & (LP_WARPS - 1)];
+#pragma unroll
+        for (int o = LP_WARPS / 2; o > 0; o >>= 1) {
+            const float oc = __shfl_xor_sync(0xffffffffu, all.c, o), os = __shfl_xor_sync(0xffffffffu, all.s, o);
+            const float ot = __shfl_xor_sync(0xffffffffu, all.t, o);
+            all.join(oc, os, ot);
+            n += __shfl_xor_sync(0xffffffffu, n, o);
+        }
+        sum = all;                                         // lane 0's is handed on below
+        ahead = n;
+    }
+    if (TOP) {
+        // the greatest 32 of two warps' sorted keys, four times
+#pragma unroll
+        for (int d = 1; d < LP_WARPS; d <<= 1) {
+            if ((warp & (2 * d - 1)) == 0) {
+                k = sorted_bitonic(greater(k, merge[warp + d][31 - lane]), lane);
+                merge[warp][lane] = k;
+            }
+            __syncthreads();
+        }
+        if (warp == 0 && lane == a.top - 1) bound_key = k;
+        __syncthreads();
+        const u64 bound = bound_key;
+        auto note = [&](u64 key) {
+            if (key < bound) return;
+            const int at = atomicAdd(&n_list, 1);
+            if (at < LP_LIST) list[at] = key;
+        };
+        if (edge >= 0) note(lp_key(xe, edge));
+        // the pieces of a thread that reaches the bound, a lane each
+        for (unsigned who = __ballot_sync(0xffffffffu, best >= bound); who; who &= who - 1) {
+            const int first = v0 + (tid & ~31) + __ffs(who) - 1;
+            for (int p = first + lane * LP_THREADS; p < v1; p += 32 * LP_THREADS) {
+                float w[N];
+                Piece<T>::load(body + (size_t)p * N, w);
+#pragma unroll
+                for (int e = 0; e < N; ++e) note(lp_key(w[e], head + p * N + e));
+            }
+        }
+        __syncthreads();
+        const int n = n_list;
+        u64* out = merge[0];                               // the slice's list, greatest first, 0 behind its end
+        if (tid < 32) out[tid] = 0;
+        __syncthreads();
+        if (n <= LP_LIST) {
+            for (int i = tid; i < n; i += LP_THREADS) {
+                const u64 key = list[i];
+                int before = 0;
+                for (int j = 0; j < n; ++j) before += list[j] > key;
+                if (before < a.top) out[before] = key;
+            }
+        } else {
+            // more than the list holds: one after the other from the logits
+            u64 below = ~0ull;
+            for (int q = 0; q < a.top; ++q) {
+                u64 mine = edge >= 0 && lp_key(xe, edge) < below ? lp_key(xe, edge) : 0;
+                for (int p = v0 + tid; p < v1; p += LP_THREADS) {
+                    float w[N];
+                    Piece<T>::load(body + (size_t)p * N, w);
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        const u64 key = lp_key(w[e], head + p * N + e);
+                        if (key < below) mine = greater(mine, key);
+                    }
+                }
+                mine = sorted(mine, lane);
+                if (lane == 0) merge[1][warp] = mine;
+                __syncthreads();
+                below = merge[1][0];
+                for (int w = 1; w < LP_WARPS; ++w) below = greater(below, merge[1][w]);
+                if (tid == 0) out[q] = below;
+                __syncthreads();
+            }
+        }
+        __syncthreads();
+    }
+    // ---- to the first CTA of the cluster
+    if (C > 1) lp_cluster_wait();
+    Slice* at = &slices[rank];
     if (tid == 0) {
-        a.logprob[row] = has ? xt - m - ls : __uint_as_float(0x7fffffffu);
-        a.entropy[row] = ls - w / s;
-        a.rank[row] = has ? (int)ahead + 1 : 0;
+        put(in_first_cta(&at->c), sum.c);
+        put(in_first_cta(&at->s), sum.s);
+        put(in_first_cta(&at->t), sum.t);
+        put(in_first_cta(&at->ahead), ahead);
     }
-    unsigned long long below = ~0ull;
-    for (int k = 0; k < a.top; ++k) {
-        unsigned long long mine = 0;
-        for (int i = tid; i < a.V; i += LP_THREADS) {
-            const unsigned long long key = lp_key(to_f32(x[i]), i);
-            if (key < below && key > mine) mine = key;
-        }
-        mine = warp_max_u64(mine);
+    if (TOP && tid < a.top) put(in_first_cta(&at->keys[tid]), merge[0][tid]);
+    if (C > 1) {
+        lp_cluster_arrive();
+        lp_cluster_wait();
+    } else {
         __syncthreads();
-        if ((tid & 31) == 0) best[tid >> 5] = mine;
-        __syncthreads();
-        below = warp_max_u64((tid & 31) < LP_THREADS / 32 ? best[tid & 31] : 0ull);
-        if (tid == 0) {
-            a.top_ids[(size_t)row * a.top + k] = (int)(0xffffffffu - (unsigned)below);
-            a.top_logprobs[(size_t)row * a.top + k] = lp_value(below) - m - ls;
+    }
+    if (rank != 0) return;
+    Sums all{slices[0].c, slices[0].s, slices[0].t};
+    int n_ahead = slices[0].ahead;
+    for (int r = 1; r < C; ++r) {
+        all.join(slices[r].c, slices[r].s, slices[r].t);
+        n_ahead += slices[r].ahead;
+    }
+    const float nan = __uint_as_float(0x7fffffffu);
+    const float ls = all.s > 0.f ? logf(all.s) : nan;     // (no softmax: NaN, or nothing but -inf)
+    if (tid == 0) {
+        a.logprob[row] = has ? xt - all.c - ls : nan;
+        a.entropy[row] = ls - all.t / all.s;
+        a.rank[row] = has ? n_ahead + 1 : 0;
+    }
+    if (TOP) {
+        // a key's place: its place in its own list and the keys ahead of it in the others
+        for (int i = tid; i < C * a.top; i += LP_THREADS) {
+            const int mine = i / a.top;
+            const u64 key = slices[mine].keys[i % a.top];
+            if (key == 0) continue;
+            int place = i % a.top;
+            for (int r = 0; r < C; ++r) {
+                if (r == mine) continue;
+                int lo = 0, hi = a.top;                    // keys ahead of it in list r
+                while (lo < hi) {
+                    const int mid = (lo + hi) / 2;
+                    if (slices[r].keys[mid] > key) lo = mid + 1;
+                    else hi = mid;
+                }
+                place += lo;
+            }
+            if (place < a.top) {
+                a.top_ids[(size_t)row * a.top + place] = (int)(0xffffffffu - (unsigned)key);
+                a.top_logprobs[(size_t)row * a.top + place] = lp_value(key) - all.c - ls;
+            }
         }
     }
+}
+
+// CTAs for a row: the least of (rounds of CTAs) x (a slice's time and what a CTA costs besides).
+int lp_cluster(int R, int V, size_t esz) {
+    int best = 1;
+    double least = 1e30;
+    for (int C = 1; C <= LP_MAX_CLUSTER; C *= 2) {
+        if (C > 1 && V < C * 2048) break;                  // a slice of some thousand logits at least
+        const long long ctas = (long long)R * C;
+        const double rounds = (double)((ctas + 295) / 296);
+        const double us = rounds * (V * (double)esz / C / 22e3 + 3.0);
+        if (us < least) {
+            least = us;
+            best = C;
+        }
+    }
+    return best;
+}
+
+template <typename T, bool TOP>
+int lp_launch(const Logprobs& a, int R, cudaStream_t stream) {
+    auto kern = logprobs_kernel<T, TOP>;
+    if (a.cluster > 8)
+        AGV_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    agv_launch_cluster(kern, dim3((unsigned)(R * a.cluster)), LP_THREADS, 0, stream, dim3(a.cluster), a);
+    AGV_LAUNCH_OK("logprobs_kernel");
+    return 0;
 }
 
 }  // namespace
@@ -105,9 +443,9 @@ AGV_API int agv_token_logprobs(const void* logits, long long ld, int dtype, int 
                 V < LP_MAX_TOP ? V : LP_MAX_TOP);
     AGV_REQUIRE(dtype == AGV_F32 || dtype == AGV_BF16, "token_logprobs: bad dtype");
     if (R == 0) return 0;
-    Logprobs a{logits, ld, V, top, tokens, logprob, entropy, rank, top_ids, top_logprobs};
-    if (dtype == AGV_F32) agv_launch(logprobs_kernel<float>, R, LP_THREADS, 0, stream, a);
-    else agv_launch(logprobs_kernel<__nv_bfloat16>, R, LP_THREADS, 0, stream, a);
-    AGV_LAUNCH_OK("logprobs_kernel");
-    return 0;
+    const int C = lp_cluster(R, V, dtype == AGV_F32 ? 4 : 2);
+    AGV_REQUIRE((long long)R * C <= 0x7fffffffLL, "token_logprobs: %d rows exceed the grid", R);
+    Logprobs a{logits, ld, V, top, C, tokens, logprob, entropy, rank, top_ids, top_logprobs};
+    if (dtype == AGV_F32) return top ? lp_launch<float, true>(a, R, stream) : lp_launch<float, false>(a, R, stream);
+    return top ? lp_launch<__nv_bfloat16, true>(a, R, stream) : lp_launch<__nv_bfloat16, false>(a, R, stream);
 }

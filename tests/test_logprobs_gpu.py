@@ -26,12 +26,13 @@ def check(logits, tokens, top):
     a = (V / 256 + 64) * 2.0 ** -24 + 2.0 ** -21 + 2.0 ** -23 * spread
     none = torch.isnan(lp)
     assert torch.equal(torch.isnan(r.logprob), none)
-    shut = torch.isinf(lp)                      # a token whose logit is -inf
-    assert torch.equal(r.logprob.double()[shut], lp[shut])
+    # (a token whose logit is -inf, or so far below the greatest that 32 bits have no number for it)
+    shut = torch.isinf(lp.float())
+    assert torch.equal(r.logprob[shut], lp.float()[shut])
     assert ((r.logprob.double() - lp).abs() <= a + 2.0 ** -22 * lp.abs())[~none & ~shut].all()
     assert ((r.entropy.double() - ent).abs() <= 3 * a * (1 + spread)).all()
-    fine = torch.isfinite(tlp)
-    assert torch.equal(r.top_logprobs.double()[~fine], tlp[~fine])
+    fine = torch.isfinite(tlp.float())
+    assert torch.equal(r.top_logprobs[~fine], tlp.float()[~fine])
     err = (r.top_logprobs.double() - tlp).abs() <= a[:, None] + 2.0 ** -22 * tlp.abs()
     assert err[fine].all()
     return r
@@ -81,6 +82,41 @@ def test_ties_orders_and_masks(dtype):
     x = torch.tensor([[1.0, 2.0, 2.0, 1.0, 2.0]], device=DEV).to(dtype)
     r = check(x, torch.tensor([4], dtype=torch.int32, device=DEV), 5)
     assert r.top_ids.tolist() == [[1, 2, 4, 0, 3]] and r.rank.tolist() == [3]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_rows_of_the_lowest_value_and_few_that_are_left(dtype):
+    """Rows that a mask has filled with the type's lowest number or -inf, all but a few places."""
+    V = 40000
+    low = float(torch.finfo(dtype).min)
+    rows = [torch.full((V,), low) for _ in range(4)] + [torch.full((V,), -math.inf) for _ in range(3)]
+    rows[1][12345] = 3.0
+    rows[2][[1, 2, 39999]] = torch.tensor([low / 2, 1.0, -5.0])
+    rows[3][::3] = float(torch.finfo(dtype).max)
+    rows[4][39999] = low
+    rows[5][[0, 7, 20000]] = torch.tensor([0.5, 0.5, -700.0])
+    rows[6][20000:20010] = -1.0
+    logits = torch.stack(rows).to(dtype).to(DEV)
+    for t in (0, 7, 12345, 39999):
+        tokens = torch.full((len(rows),), t, dtype=torch.int32, device=DEV)
+        for top in (0, 3, 20, 32):
+            if t == 7 or top in (0, 20):
+                check(logits, tokens, top)
+
+
+def test_the_greatest_all_in_one_place():
+    """Descending and equal runs whose greatest logits are all one thread's or one piece's, and more of
+    them than are kept in a list."""
+    V = 3_000_000
+    x = -torch.rand(1, V, generator=torch.Generator().manual_seed(4)).to(DEV)
+    for stride in (1, 2048, 4096, 1 << 16):
+        y = x.clone()
+        y[0, 1000::stride][:1400] += 5
+        check(y, torch.tensor([1000], dtype=torch.int32, device=DEV), 32)
+    y = x.clone()
+    for q in range(32):                                  # 32 threads' shares
+        y[0, q * 4::2048] += 5
+    check(y, torch.tensor([5], dtype=torch.int32, device=DEV), 32)
 
 
 def test_rows_without_a_softmax_and_tokens_outside():
