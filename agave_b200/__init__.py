@@ -15,7 +15,7 @@ def __getattr__(name):
     if name == "Engine":
         from .engine.api import Engine
         return Engine
-    if name == "SamplingParams":
-        from .sampling import SamplingParams
-        return SamplingParams
+    if name in ("SamplingParams", "TokenScore"):
+        from . import sampling
+        return getattr(sampling, name)
     raise AttributeError(name)

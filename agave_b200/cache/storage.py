@@ -73,6 +73,7 @@ class Cache:
         if kv_dtype == torch.float8_e4m3fn and not any(g.codes for g in groups):
             raise CacheError("no layer of this model holds keys and values that 8-bit codes can stand "
                              "for")
+        self.codes = any(g.codes for g in groups)      # whether any entry is held in 8 bits
         self.book = CacheBook(groups, n_slots, max_seq_len)
         self.n_slots = n_slots
         self.k_pools: List[torch.Tensor] = []

@@ -8,10 +8,10 @@ Option names and meanings are the reference's where it has them
 ``--repeat-penalty`` (1.0), ``--seed`` (random), ``--ctx-size`` (0 = the model's
 own limit; default min(model, 4096)), ``-q/--quiet``, ``--json``,
 ``--model-info``, ``-V/--verbose``, ``-d/--debug``, ``-v/--version``.
-Options of what this library does not have (other backends, quantised caches,
-server, vision, speculative decoding, grammars) are not offered.  Added here:
+Options of what this library does not have (other backends, caches quantised below 8 bits, server, vision, speculative decoding, grammars) are not offered.  Added here:
 ``--tokens`` (a prompt as token ids), ``--dtype``, ``--max-batch``,
-``--random-weights SEED`` (the folder then needs only ``config.json``: seeded random
+``--logprobs N`` and ``--score`` (log-probabilities of the tokens generated, or of the
+prompt's own), ``--random-weights SEED`` (the folder then needs only ``config.json``: seeded random
 weights are drawn on the device) and ``--strict`` (refuse folders that hold tensors the
 decoder does not ask for).  ``--profile`` prints the reference's per-operation table
 (src/perf.zig:84-130), with device times, for a run whose steps go launch by launch.
@@ -25,6 +25,7 @@ from __future__ import annotations
 
 import argparse
 import json
+import math
 import os
 import sys
 import time
@@ -111,6 +112,11 @@ def build_parser() -> argparse.ArgumentParser:
                    help="Repetition penalty [default: 1.0].")
     g.add_argument("--seed", type=int, default=None,
                    help="Random seed for sampling [default: random].")
+    g.add_argument("--logprobs", type=int, default=None, metavar="N",
+                   help="Log-probability, entropy and rank of every generated token, with the N (0 to 32) "
+                        "most likely ones (printed with --json).")
+    g.add_argument("--score", action="store_true",
+                   help="Generate nothing: log-probabilities of the prompt's own tokens.")
     g.add_argument("--system", default=None, help="System prompt for chat formatting.")
     g.add_argument("--tokens", default=None,
                    help="Prompt as comma-separated token ids; several prompts separated by ';'.")
@@ -141,7 +147,8 @@ def build_parser() -> argparse.ArgumentParser:
     g.add_argument("--allow-cpu-fallback", action="store_true", help="Refused: there is no CPU path.")
     g.add_argument("--kv-type", default=None,
                    help="Cache element type: bf16 (f16 is read as bf16) with --dtype bfloat16, f32 "
-                        "with --dtype float32; quantised caches are refused.")
+                        "with --dtype float32, or e4m3 (fp8): 8-bit codes with a scale per page and "
+                        "head; other quantised caches are refused.")
     for name in ("--kv-type-k", "--kv-type-v", "--cache-type-k", "--cache-type-v"):
         g.add_argument(name, default=None, help="As --kv-type.")
     for name, why in (("--kv-tiers", "tiered caches"), ("--kv-eviction", "cache eviction"),
@@ -186,6 +193,15 @@ def _fail(msg: str) -> int:
     return 1
 
 
+KV_CODES = ("e4m3", "fp8", "f8", "fp8_e4m3", "f8e4m3")
+
+
+def _holds_codes(args) -> bool:
+    """Whether the options ask for the 8-bit cache (after ``_unsupported`` has passed them)."""
+    return any((getattr(args, n) or "").lower() in KV_CODES
+               for n in ("kv_type", "kv_type_k", "cache_type_k"))
+
+
 def _unsupported(args) -> Optional[str]:
     """Why an option of the reference's command line cannot be honoured here, or None."""
     if args.backend not in ("auto", "cuda"):
@@ -194,11 +210,21 @@ def _unsupported(args) -> Optional[str]:
         return "--allow-cpu-fallback: there is no CPU path"
     want = {"bfloat16": ("bf16", "f16", "fp16", "bfloat16", "float16"),
             "float32": ("f32", "fp32", "float32")}[args.dtype]
+    codes = []
     for name in ("kv_type", "kv_type_k", "kv_type_v", "cache_type_k", "cache_type_v"):
         v = getattr(args, name)
-        if v is not None and v.lower() not in want:
+        if v is not None and v.lower() not in want + KV_CODES:
             return (f"--{name.replace('_', '-')} {v}: the cache holds {args.dtype} with --dtype "
-                    f"{args.dtype}; there are no quantised or mixed caches")
+                    f"{args.dtype}, or e4m3; there are no other quantised and no mixed caches")
+        if v is not None:
+            codes.append(v.lower() in KV_CODES)
+    if any(codes) and not (args.kv_type is not None and all(codes)):
+        # keys and values are held alike: e4m3 by --kv-type, or by the options of both
+        ks = [n for n in ("kv_type_k", "cache_type_k") if (getattr(args, n) or "").lower() in KV_CODES]
+        vs = [n for n in ("kv_type_v", "cache_type_v") if (getattr(args, n) or "").lower() in KV_CODES]
+        if not (all(codes) and ks and vs):
+            return ("--kv-type: keys and values are both e4m3 or both "
+                    f"{args.dtype}; there are no mixed caches")
     for name, why in (("kv_tiers", "tiered caches"), ("kv_eviction", "cache eviction"),
                       ("grammar", "constrained decoding"), ("grammar_string", "constrained decoding"),
                       ("json_output", "constrained decoding"), ("draft_model", "speculative decoding"),
@@ -208,6 +234,39 @@ def _unsupported(args) -> Optional[str]:
         if v not in (None, False) and not (name == "kv_eviction" and v == "none"):
             return f"--{name.replace('_', '-')}: this library has no {why}"
     return None
+
+
+def _number(v: float):
+    return v if math.isfinite(v) else None          # (JSON has no infinities)
+
+
+def _score_record(s) -> dict:
+    return {"id": s.token, "logprob": _number(s.logprob), "entropy": _number(s.entropy),
+            "rank": s.rank, "top": [[i, _number(lp)] for i, lp in s.top]}
+
+
+def _score_prompts(engine, prompts, args) -> int:
+    """``--score``: what the model gives the prompts' own tokens."""
+    try:
+        scores = engine.score(prompts, top=args.logprobs or 0)
+    except (ValueError, RuntimeError) as e:
+        return _fail(str(e))
+    recs = []
+    for p, row in zip(prompts, scores):
+        total = sum(s.logprob for s in row)
+        mean = total / len(row) if row else 0.0
+        recs.append({"tokens": len(p), "logprob_sum": _number(total),
+                     "perplexity": _number(math.exp(min(-mean, 700.0))),
+                     "logprobs": [_score_record(s) for s in row]})
+    if args.json:
+        print(json.dumps(recs[0] if len(recs) == 1 else recs))
+        return 0
+    for p, row, rec in zip(prompts, scores, recs):
+        for s in row:
+            print(f"{s.token}\t{s.logprob:.6f}\t{s.rank}")
+        if not args.quiet:
+            print(f"{rec['tokens']} tok · perplexity {rec['perplexity']}", file=sys.stderr)
+    return 0
 
 
 def main(argv: Optional[List[str]] = None) -> int:
@@ -234,6 +293,8 @@ def main(argv: Optional[List[str]] = None) -> int:
         return _fail("--repeat-penalty must be > 0")
     if args.max_tokens < 0:
         return _fail("--max-tokens must be >= 0")
+    if args.logprobs is not None and not 0 <= args.logprobs <= 32:
+        return _fail("--logprobs must lie in 0..32")
     args.verbose = args.verbose or args.debug
     quiet = args.quiet or args.json
 
@@ -294,7 +355,7 @@ def main(argv: Optional[List[str]] = None) -> int:
     max_batch = args.max_batch or n
     t0 = time.time()
     sizes = dict(dtype=args.dtype, max_tokens=max_batch * ((ctx + 63) // 64 * 64), ctx_size=ctx,
-                 max_batch=max_batch)
+                 max_batch=max_batch, cache_dtype="e4m3" if _holds_codes(args) else None)
     try:
         if args.random_weights is not None:
             engine = Engine.from_config(raw_config, seed=args.random_weights, **sizes)
@@ -302,6 +363,8 @@ def main(argv: Optional[List[str]] = None) -> int:
             engine = Engine(args.model, strict=args.strict, **sizes)
     except (WeightsError, SafetensorsError, ConfigError, RuntimeError) as e:
         return _fail(str(e))
+    if args.score and not args.model_info:
+        return _score_prompts(engine, prompts, args)
     info = engine.model_info()
     c = info["config"]
     if args.model_info:
@@ -343,7 +406,7 @@ def main(argv: Optional[List[str]] = None) -> int:
         outs = engine.generate(prompts, max_new_tokens=args.max_tokens,
                                temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
                                repeat_penalty=args.repeat_penalty, seed=args.seed,
-                               stop_token_ids=stops)
+                               stop_token_ids=stops, logprobs=args.logprobs)
     except (ValueError, RuntimeError) as e:
         return _fail(str(e))
     finally:
@@ -370,6 +433,9 @@ def main(argv: Optional[List[str]] = None) -> int:
                "prefill_tok_per_sec": st["prefill_tokens"] / st["prefill_seconds"]
                if st["prefill_seconds"] > 0 else 0.0,
                "gen_ms": gen_ms}
+        if engine.logprobs is not None:
+            lps = [[_score_record(s) for s in o] for o in engine.logprobs]
+            rec["logprobs"] = lps[0] if len(lps) == 1 else lps
         print(json.dumps(rec))
     else:
         for t in texts:

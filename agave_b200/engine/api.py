@@ -5,7 +5,8 @@ token ids out.
     outs = engine.generate([[2, 17, 5], [2, 9]], max_new_tokens=32)
 
 ``Engine.step`` is the step function that trace replay drives; ``generate``
-is the loop above it.  Decode steps of ``generate`` are recorded once per
+is the loop above it, ``score`` gives the log-probability of every token of given
+sequences.  ``cache_dtype="e4m3"`` holds keys and values in 8 bits.  Decode steps of ``generate`` are recorded once per
 batch size as a CUDA graph and replayed; per step the host writes the batch's
 token ids, positions and slots into pinned memory, copies them to the graph's
 fixed input buffers and reads the chosen tokens back.
@@ -27,7 +28,7 @@ from .. import kernels
 from ..cache import PAGE, CacheError, round_up
 from ..config import load_config, resolve_architecture
 from ..models.decoder import DecoderModel, decoder_param_specs
-from ..sampling import Sampler, SamplingParams
+from ..sampling import Sampler, SamplingParams, TokenScore
 from ..weights import head_is_stored, load_weights, random_tensors
 from .batch import DECODE, PREFILL, Cancelled, StepContext
 from .generate import GenerationPlan, RequestState
@@ -35,6 +36,9 @@ from .step import Runner, StepError
 
 _DTYPES = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16,
            "float32": torch.float32, "fp32": torch.float32, "f32": torch.float32}
+# names of the 8-bit cache (a cache in the compute dtype goes by that one's names)
+_CODES = {"e4m3", "fp8", "f8", "fp8_e4m3", "f8e4m3", "float8_e4m3fn"}
+SCORE_LOGITS = 1 << 26        # logits that ``score`` holds at a time
 
 
 def _bucket(n: int) -> int:
@@ -47,14 +51,24 @@ def _bucket(n: int) -> int:
     return round_up(n, 8)
 
 
+def cache_dtype_of(name: Optional[str], dtype: torch.dtype) -> Optional[torch.dtype]:
+    """The element type of a cache by its name (None: the compute dtype)."""
+    if name is None or _DTYPES.get(name) == dtype:
+        return None
+    if name in _CODES:
+        return kernels.E4M3
+    raise ValueError(f"cache_dtype {name!r} is not supported (the compute dtype, or e4m3)")
+
+
 class _DecodeGraph:
     """One recorded decode step for a padded batch size and a kind of choice (arg
-    max or a draw, with or without the repeat penalty).  The sampling options
+    max or a draw, with or without the repeat penalty, with or without log-probabilities).  The sampling options
     themselves (temperature, top_k, top_p, seed, penalty) are step inputs on the
     device, so one recording serves every setting of its kind."""
 
-    def __init__(self, engine: "Engine", size: int, params: SamplingParams, seed: int):
-        self.size = size
+    def __init__(self, engine: "Engine", size: int, params: SamplingParams, seed: int,
+                 top: Optional[int] = None):
+        self.size, self.top = size, top
         dev = engine.device
         B = size
         n_int = round_up(3 * B + 3 * B + 1 + B + 1, 2)  # step arrays, sampling steps, flag; even
@@ -83,6 +97,10 @@ class _DecodeGraph:
         # before the result of the step before it has been read
         self.next_hosts = [torch.zeros(B, dtype=torch.int32, pin_memory=True) for _ in range(2)]
         self.done = [torch.cuda.Event() for _ in range(2)]
+        self.scores: Optional[kernels.TokenLogprobs] = None
+        self.score_hosts = [None, None]
+        if top is not None:
+            self.score_hosts = [torch.zeros((3 + 2 * top) * B, pin_memory=True) for _ in range(2)]
         self.logits: Optional[torch.Tensor] = None
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.kernels_per_step = 0
@@ -100,13 +118,19 @@ class _DecodeGraph:
                           max_len=runner.cache.max_seq_len, max_new=1, cache=runner.cache,
                           dtype=runner.dtype, device=runner.device, lens_host=lens_host)
         engine.sampler.note_inputs(v["tokens"], v["slots"])
-        fused = params.greedy and params.repeat_penalty == 1.0 and engine.fused_greedy
+        fused = (params.greedy and params.repeat_penalty == 1.0 and engine.fused_greedy and
+                 self.top is None)
         self.logits = runner.model.run_step(ctx, self.rows,
                                             choose_into=self.next_dev if fused else None)
         if self.logits is None:
             return                     # the greatest logit was found in the head's epilogue
+        raw = self.logits
+        if self.top is not None and params.repeat_penalty != 1.0:
+            raw = raw.clone()          # (the penalty changes the logits in place)
         engine.sampler.choose(self.logits, self.next_dev, params, seed, v["slots"], self.seq_ids,
                               v["steps"], penalise=True, dev_params=self.words)
+        if self.top is not None:
+            self.scores = kernels.token_logprobs(raw, self.next_dev, self.top)
 
     def _record(self, engine: "Engine", params: SamplingParams, seed: int) -> None:
         if not engine.use_graphs:
@@ -145,6 +169,8 @@ class _DecodeGraph:
         else:
             self._body(engine, params, seed)
         self.next_hosts[which].copy_(self.next_dev, non_blocking=True)
+        if self.top is not None:
+            self.score_hosts[which].copy_(self.scores.packed, non_blocking=True)
         self.done[which].record()
 
     def wait(self, which: int = 0) -> "np.ndarray":
@@ -152,9 +178,20 @@ class _DecodeGraph:
         self.done[which].synchronize()
         return self.next_hosts[which].numpy()
 
+    def token_scores(self, which: int):
+        """The log-probabilities that came with those tokens (after ``wait``)."""
+        return kernels.TokenLogprobs.unpack(self.score_hosts[which].numpy(), self.size, self.top)
+
     def run(self, engine: "Engine", params: SamplingParams, seed: int) -> None:
         self.launch(engine, params, seed)
         self.wait()
+
+
+def _score(token: int, found, row: int) -> TokenScore:
+    """Row ``row`` of unpacked log-probabilities as a record."""
+    lp, ent, rank, ids, lps = found
+    return TokenScore(int(token), float(lp[row]), float(ent[row]), int(rank[row]),
+                      tuple(zip(ids[row].tolist(), lps[row].tolist())))
 
 
 class Engine:
@@ -163,9 +200,11 @@ class Engine:
     def __init__(self, model_dir: Optional[str] = None, *, dtype: str = "bfloat16",
                  max_tokens: int = 65536, ctx_size: int = 0, max_batch: Optional[int] = None,
                  device: str = "cuda:0", use_graphs: bool = True, strict: bool = False,
+                 cache_dtype: Optional[str] = None,
                  _raw_config: Optional[dict] = None, _tensors: Optional[dict] = None):
         if dtype not in _DTYPES:
             raise ValueError(f"dtype {dtype!r} is not supported (bfloat16, float32)")
+        kv_dtype = cache_dtype_of(cache_dtype, _DTYPES[dtype])
         if not torch.cuda.is_available():
             raise RuntimeError("agave_b200 needs a CUDA device: there is no CPU path")
         self.device = torch.device(device)
@@ -207,13 +246,14 @@ class Engine:
             max_batch = max(1, min(1024, round_up(max_tokens, PAGE) // PAGE))
         self.max_batch, self.max_tokens = max_batch, max_tokens
         self.runner = Runner(self.model, max_tokens, max_seq_len, max_batch,
-                             use_graphs=use_graphs)
+                             use_graphs=use_graphs, kv_dtype=kv_dtype)
         self.max_seq_len = self.runner.cache.max_seq_len
         self.sampler = Sampler(max_batch, self.device)
         kernels.prepare_device(self.device)
         self.use_graphs = use_graphs
         self._graphs: Dict[Tuple, _DecodeGraph] = {}
         self.stats: Dict[str, float] = {}
+        self.logprobs: Optional[List[List[TokenScore]]] = None
         # greedy decoding takes the arg max in the head product's epilogue
         self.fused_greedy = os.environ.get("AGAVE_B200_FUSED_GREEDY", "1") != "0"
         self._cancel = threading.Event()
@@ -262,13 +302,18 @@ class Engine:
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int = 512,
                  temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0,
                  repeat_penalty: float = 1.0, seed: Optional[int] = None,
-                 stop_token_ids: Optional[Sequence[int]] = None) -> List[List[int]]:
+                 stop_token_ids: Optional[Sequence[int]] = None,
+                 logprobs: Optional[int] = None) -> List[List[int]]:
         """Token ids generated for each prompt (stop tokens excluded).
 
         Option names and defaults are the reference's (src/main.zig:333-338):
         temperature 0 is greedy.  ``stop_token_ids`` defaults to the
-        configuration's end-of-sequence ids.
+        configuration's end-of-sequence ids.  ``logprobs`` N (0 to 32): ``self.logprobs`` then
+        holds a ``TokenScore`` for every token returned, with the N most likely in its place.
         """
+        if logprobs is not None and not 0 <= logprobs <= min(kernels.LOGPROBS_MAX_TOP,
+                                                             self.spec.vocab_size):
+            raise ValueError(f"logprobs must lie in 0..{kernels.LOGPROBS_MAX_TOP}")
         params = SamplingParams(temperature, top_k, top_p, repeat_penalty, seed).validate()
         seed_v = 0 if params.greedy else params.resolved_seed()
         stops = self.spec.eos_token_ids if stop_token_ids is None else tuple(stop_token_ids)
@@ -276,6 +321,7 @@ class Engine:
                               self.max_seq_len)
         stats = dict(prefill_tokens=0, prefill_seconds=0.0, decode_tokens=0, decode_seconds=0.0,
                      decode_steps=0, batches=0)
+        scores = None if logprobs is None else [[] for _ in prompts]
         try:
             while True:
                 batch = plan.next_batch()
@@ -283,7 +329,7 @@ class Engine:
                     break
                 stats["batches"] += 1
                 try:
-                    self._run_batch(plan, batch, params, seed_v, stats)
+                    self._run_batch(plan, batch, params, seed_v, stats, logprobs, scores)
                 except Cancelled:
                     plan.cancel()
                 if self._cancel.is_set():
@@ -292,10 +338,60 @@ class Engine:
             self._cancel.clear()
         self.stats = stats
         self.finish_reasons = [r.finish_reason for r in plan.requests]
+        self.logprobs = scores
         return plan.outputs()
 
+    def score(self, sequences: Sequence[Sequence[int]], top: int = 0) -> List[List[TokenScore]]:
+        """What the model gives every token of each sequence after its first, from the tokens before
+        it: one ``TokenScore`` each (their sum of log-probabilities is the sequence's).
+
+        Sequences run whole, as prompts do, as many at a time as the cache holds; the logits of
+        some rows at a time are formed and read, so no whole [tokens, vocabulary] is held."""
+        if not 0 <= top <= min(kernels.LOGPROBS_MAX_TOP, self.spec.vocab_size):
+            raise ValueError(f"top must lie in 0..{kernels.LOGPROBS_MAX_TOP}")
+        plan = GenerationPlan(sequences, 1, (), self.max_batch, self.max_tokens, self.max_seq_len)
+        out: List[List[TokenScore]] = [[] for _ in sequences]
+        try:
+            while True:
+                batch = plan.next_batch()
+                if not batch:
+                    return out
+                self._score_batch(batch, top, out)
+                plan.accept({r.index: 0 for r in batch})
+        except Cancelled:
+            self._cancel.clear()
+            raise
+
+    def _score_batch(self, batch, top: int, out: List[List[TokenScore]]) -> None:
+        for r in batch:
+            r.slot = self.acquire()
+        try:
+            ctx = self.runner.context([(r.slot, r.prompt) for r in batch])
+            ctx.cancel = self._cancel
+            h = self.model.hidden_states(ctx)
+            rows, targets, owners, at = [], [], [], 0
+            for r in batch:
+                n = len(r.prompt)
+                rows.extend(range(at, at + n - 1))
+                targets.extend(r.prompt[1:])
+                owners.extend([r.index] * (n - 1))
+                at += n
+            both = torch.tensor([rows, targets], dtype=torch.int32).to(self.device)
+            step = max(1, SCORE_LOGITS // self.spec.vocab_size)
+            for a in range(0, len(rows), step):
+                logits = self.model.logits(h, both[0, a:a + step], ctx)
+                found = kernels.token_logprobs(logits, both[1, a:a + step], top)
+                n = logits.shape[0]
+                host = kernels.TokenLogprobs.unpack(found.packed.cpu().numpy(), n, top)
+                for i in range(n):
+                    out[owners[a + i]].append(_score(targets[a + i], host, i))
+        finally:
+            for r in batch:
+                self.release(r.slot)
+                r.slot = -1
+
     def _run_batch(self, plan: GenerationPlan, batch, params: SamplingParams, seed: int,
-                   stats: dict) -> None:
+                   stats: dict, top: Optional[int] = None, scores=None) -> None:
         dev = self.device
         for r in batch:
             r.slot = self.acquire()
@@ -312,15 +408,22 @@ class Engine:
             self.sampler.choose(logits, first, params, seed, slots, seq_ids, steps,
                                 penalise=False)
             first_host = first.cpu()
+            found = None
+            if top is not None:
+                # (the first choice is made without a penalty: the logits are as they were)
+                found = kernels.TokenLogprobs.unpack(
+                    kernels.token_logprobs(logits, first, top).packed.cpu().numpy(), B, top)
             stats["prefill_seconds"] += time.perf_counter() - t0
             stats["prefill_tokens"] += sum(len(r.prompt) for r in batch)
             ended = plan.accept({r.index: int(first_host[i]) for i, r in enumerate(batch)})
+            if found is not None:
+                self._note_scores(list(enumerate(batch)), found, scores)
             for r in ended:
                 self.release(r.slot)
                 r.slot = -1
             # one token each until the batch is empty
             t0 = time.perf_counter()
-            self._decode_loop(plan, params, seed, stats)
+            self._decode_loop(plan, params, seed, stats, top, scores)
             stats["decode_seconds"] += time.perf_counter() - t0
         finally:
             for r in batch:
@@ -328,23 +431,32 @@ class Engine:
                     self.release(r.slot)
                     r.slot = -1
 
-    def _graph_for(self, size: int, params: SamplingParams, seed: int) -> _DecodeGraph:
+    @staticmethod
+    def _note_scores(rows, found, scores) -> None:
+        """Keeps the records of the tokens that the requests (row, request) have just taken."""
+        for i, r in rows:
+            if len(r.output) > len(scores[r.index]):           # (a stop token is not returned)
+                scores[r.index].append(_score(r.output[-1], found, i))
+
+    def _graph_for(self, size: int, params: SamplingParams, seed: int,
+                   top: Optional[int] = None) -> _DecodeGraph:
         # what is fixed in a recording: the padded batch and which kernels choose the token
-        key = (size, params.greedy, params.repeat_penalty != 1.0)
+        key = (size, params.greedy, params.repeat_penalty != 1.0, top)
         g = self._graphs.get(key)
         if g is None:
             if len(self._graphs) >= 64:
                 self._graphs.clear()
-            g = self._graphs[key] = _DecodeGraph(self, size, params, seed)
+            g = self._graphs[key] = _DecodeGraph(self, size, params, seed, top)
         return g
 
-    def _stage_step(self, live, params: SamplingParams, seed: int, ahead: int, which: int):
+    def _stage_step(self, live, params: SamplingParams, seed: int, ahead: int, which: int,
+                    top: Optional[int] = None):
         """Fill staging buffer ``which`` of the live set's graph with everything a
         decode step needs except the token ids, for the step ``ahead`` steps after
         the last committed one; reserves the cache rows it will write."""
         n = len(live)
         B = _bucket(n)
-        g = self._graph_for(B, params, seed)
+        g = self._graph_for(B, params, seed, top)
         book = self.runner.cache.book
         for r in live:
             self.runner.cache.reserve(r.slot, book.length[r.slot] + ahead + 1)
@@ -369,7 +481,7 @@ class Engine:
         return g
 
     def _decode_loop(self, plan: GenerationPlan, params: SamplingParams, seed: int,
-                     stats: dict) -> None:
+                     stats: dict, top: Optional[int] = None, scores=None) -> None:
         """One token for every live sequence per step until the batch is empty.
 
         A step is launched before the host has read the step before it (its token
@@ -394,7 +506,7 @@ class Engine:
                 return
             if inflight is None:
                 n = len(live)
-                g = self._stage_step(live, params, seed, 0, which)
+                g = self._stage_step(live, params, seed, 0, which, top)
                 g.hosts_np[which][:n] = np.fromiter((r.output[-1] for r in live), dtype=np.int32,
                                                     count=n)
                 g.hosts_np[which][g.flag_at] = 0
@@ -407,7 +519,7 @@ class Engine:
             if (not self._cancel.is_set() and
                     all(not r.done and len(r.output) + 1 < r.max_new for r in reqs)):
                 try:
-                    g2 = self._stage_step(reqs, params, seed, 1, 1 - w)
+                    g2 = self._stage_step(reqs, params, seed, 1, 1 - w, top)
                     g2.hosts_np[1 - w][g2.flag_at] = 1
                     cache.flush()
                     g2.launch(self, params, seed, 1 - w)
@@ -422,6 +534,8 @@ class Engine:
             stats["decode_steps"] += 1
             stats["decode_tokens"] += len(current)
             ended = plan.accept(sampled)
+            if top is not None:
+                self._note_scores(current, g.token_scores(w), scores)
             if ahead is not None:
                 held.extend(ended)
                 inflight = ahead

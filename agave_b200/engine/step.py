@@ -46,14 +46,14 @@ class Runner:
     """A model with its cache and its recorded prompt steps; owns nothing else."""
 
     def __init__(self, model, max_tokens: int, max_seq_len: int, n_slots: int,
-                 use_graphs: bool = True):
+                 use_graphs: bool = True, kv_dtype: Optional[torch.dtype] = None):
         self.use_graphs = use_graphs
         self._prompt_graphs: "OrderedDict[tuple, _PromptGraph]" = OrderedDict()
         self._prompt_seen: dict = {}
         self.model = model
         self.device, self.dtype = model.device, model.dtype
         self.cache = Cache(model.cache_requests(), max_tokens, max_seq_len, n_slots,
-                           model.dtype, model.device)
+                           model.dtype, model.device, kv_dtype)
         self.cancel_flag = None        # a threading.Event an eager step checks between blocks
         self.vocab_size = model.spec.vocab_size
 

@@ -2146,7 +2146,17 @@ class TokenLogprobs:
     """What ``token_logprobs`` finds for R rows: ``logprob`` and ``entropy`` [R] (32-bit, nats),
     ``rank`` [R] (int32; 1 = the greatest logit), ``top_ids`` [R, top] (int32) and
     ``top_logprobs`` [R, top] (32-bit), greatest first, equal ones by index."""
-    __slots__ = ("logprob", "entropy", "rank", "top_ids", "top_logprobs")
+    __slots__ = ("logprob", "entropy", "rank", "top_ids", "top_logprobs", "packed")
+
+    # ``packed``: all of it, 32 bits a value, in this order, so that one copy brings it to the host
+    @staticmethod
+    def unpack(packed, rows: int, top: int):
+        """(logprob, entropy, rank, top ids, top logprobs) of a host copy of ``packed`` (numpy)."""
+        import numpy as np
+        i = packed.view(np.int32)
+        ids, lps = i[3 * rows:(3 + top) * rows], packed[(3 + top) * rows:(3 + 2 * top) * rows]
+        return (packed[:rows], packed[rows:2 * rows], i[2 * rows:3 * rows], ids.reshape(rows, top),
+                lps.reshape(rows, top))
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
@@ -2169,6 +2179,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     r.logprob, r.entropy, r.rank = floats[:R], floats[R:2 * R], ints[2 * R:3 * R]
     r.top_ids = ints[3 * R:(3 + top) * R].view(R, top)
     r.top_logprobs = floats[(3 + top) * R:].view(R, top)
+    r.packed = floats
     with _span("token_logprobs", _nbytes(logits, floats)):
         _check(library().agv_token_logprobs(
             _ptr(logits), ctypes.c_longlong(logits.stride(0)), dtype_code(logits.dtype), R, V,

@@ -161,6 +161,7 @@ class DecoderModel:
         dot products with the joins in their prologues (``kernels.gemv_few``)."""
         T = ctx.n_tokens
         if ctx.mode != DECODE or not self.standard or self.dtype != torch.bfloat16 or \
+                getattr(ctx.cache, "codes", False) or \
                 not 1 <= T <= kernels.FEW_TOKENS or not self.spec.schedule:
             return False
         H = self.spec.hidden_size
@@ -318,15 +319,16 @@ class DecoderModel:
         returned and nothing is chosen).
 
         Models of standard blocks take the C++ host path (one call into the library for
-        the whole step); others, and any step whose operations are being timed, run
-        through the Python parts launch by launch."""
+        the whole step); others, a cache that holds 8-bit codes, and any step whose operations
+        are being timed, run through the Python parts launch by launch."""
         n_rows = rows.numel() if rows is not None else 0
         if ctx.cancel is not None and ctx.cancel.is_set():
             raise Cancelled("cancelled before the step")
         greedy = (choose_into is not None and n_rows > 0 and self.dtype == torch.bfloat16 and
                   n_rows <= kernels.ARGMAX_MAX_ROWS and self.spec.hidden_size % 8 == 0 and
                   self.head.weight.data_ptr() % 16 == 0)
-        if self.native is not None and kernels._perf is None and not kernels.NVTX:
+        if self.native is not None and kernels._perf is None and not kernels.NVTX and \
+                not getattr(ctx.cache, "codes", False):
             if n_rows == 0:
                 self.native.run(ctx, None)
                 return None

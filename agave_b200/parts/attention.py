@@ -20,6 +20,11 @@ the norm, the rotation and that store itself).  A call
 that does not write the cache reads what the owning call stored: during a
 prompt step through ``ctx.step_kv``, during decoding through the cache.
 
+A cache entry that holds 8-bit codes is filled by a store of its own after the norm and the
+rotation, and read by a decode attention of its own (``kernels.cache_store_e4m3``,
+``attention_decode_e4m3``); prompts attend from the step's tensors as ever, so a prompt's
+outputs are those of a cache in the compute dtype.
+
 Options of the spec, each a parameter of the kernels: value heads of another size
 than the keys' (``value_dim``), a sink logit per query head that joins the softmax
 denominator once (``sink``; tensor ``sink``), a query temperature that multiplies q by
@@ -203,7 +208,8 @@ class AttentionMixer:
         if self.keep_first or getattr(self.spec, "keep_all_keys", False):
             window = None
         kv = KVRequest(self.spec.n_kv_heads, self.spec.head_dim, window,
-                       0 if self.value_dim == self.spec.head_dim else self.value_dim)
+                       0 if self.value_dim == self.spec.head_dim else self.value_dim,
+                       eight_bit=kernels.e4m3_head_supported(self.spec.head_dim, self.value_dim))
         st = self.state_request()
         return kv if st is None else (kv, st)
 
@@ -286,6 +292,14 @@ class AttentionMixer:
         if self.value_mix is not None and self.value_mix.source is not None:
             self.mix_weight = float(tensors["value_mix"].to(torch.float32).reshape(()).item())
 
+    def _store_codes(self, qkv: torch.Tensor, view, ctx) -> None:
+        """The step's keys and values, from a row q | k | v, into a cache entry of 8-bit codes."""
+        s = self.spec
+        k0 = s.n_heads * s.head_dim
+        v0 = k0 + s.n_kv_heads * s.head_dim
+        kernels.cache_store_e4m3(qkv[:, k0:v0], qkv[:, v0:v0 + s.n_kv_heads * self.value_dim], view,
+                                 ctx, s.n_kv_heads, s.head_dim, value_dim=self.value_dim)
+
     def forward_terms(self, x: torch.Tensor, ctx, cache_entry: int, writes_cache: bool):
         """The branch as terms of a sum with their multipliers, for a block that joins them
         itself: the output product and, where there is one, its bias (one row for all)."""
@@ -315,6 +329,7 @@ class AttentionMixer:
             cos, sin = self.position.tables(ctx)
             rotary_dim = self.position.rotary_dim
         view = ctx.cache.kv_view(cache_entry)
+        codes = view.k_scale is not None      # held in 8 bits: a store and an attention of their own
         eps = s.qk_norm.eps if s.qk_norm is not None else 0.0
         window = s.window or 0
         if ctx.mode == PREFILL and kernels.qkv_prefill_supported(x, self.qkv.weight, hd,
@@ -328,14 +343,16 @@ class AttentionMixer:
                 vt = kernels.prefill_values_scratch(T, ctx.batch, nkv, hd, qkv.device)
             pools = dict(k_pool=view.k_pool, v_pool=view.v_pool, page_table=view.page_table,
                          slots=ctx.slots, lens=ctx.lens, page=view.page,
-                         cap=view.cap) if writes_cache else {}
+                         cap=view.cap) if writes_cache and not codes else {}
             kernels.qkv_prefill(x, self.qkv.weight, qkv, nh, nkv, hd, self.q_norm_weight,
                                 self.k_norm_weight, eps, cos, sin, ctx.positions, ctx.seq_index,
                                 vt=vt, cu_seqlens=ctx.cu_seqlens, **pools)
+            if writes_cache and codes:
+                self._store_codes(qkv, view, ctx)
             return self._attend_prompt(qkv, vt, ctx, cache_entry, writes_cache, window)
         proj = self.qkv.partial(x, cheap_sum=True)
         part = proj if proj.dim() == 3 else None
-        if (ctx.mode == DECODE and part is not None and
+        if (ctx.mode == DECODE and part is not None and not codes and
                 kernels.attention_decode_fused_supported(self.dtype, hd, rotary_dim)):
             # decoding: norm, rotation and the store of the new key and value happen inside
             # the attention kernel, on the projection's partial sums
@@ -352,11 +369,14 @@ class AttentionMixer:
             if ctx.mode == PREFILL and kernels.attention_prefill_wants_transposed_values(
                     qkv, ctx, nh, nkv, hd):
                 vt = kernels.prefill_values_scratch(T, ctx.batch, nkv, hd, qkv.device)
+            pools = (view.k_pool, view.v_pool) if not codes else (None, None)
             kernels.qk_norm_rope_store(
                 qkv, nh, nkv, hd, self.q_norm_weight, self.k_norm_weight, eps, cos, sin,
-                rotary_dim, ctx.positions, view.k_pool, view.v_pool, view.page_table, ctx.slots,
+                rotary_dim, ctx.positions, *pools, view.page_table, ctx.slots,
                 ctx.lens, ctx.seq_index, view.page, view.cap, partial=part, vt=vt,
                 cu_seqlens=ctx.cu_seqlens, max_len=ctx.max_new)
+            if codes:
+                self._store_codes(qkv, view, ctx)
         else:
             kernels.qk_norm_rope_store(qkv, nh, nkv, hd, self.q_norm_weight, self.k_norm_weight,
                                        eps, cos, sin, rotary_dim, ctx.positions, partial=part)
@@ -385,6 +405,7 @@ class AttentionMixer:
             cos, sin = self.position.tables(ctx)
             rotary_dim = self.position.rotary_dim
         view = ctx.cache.kv_view(cache_entry)
+        codes = view.k_scale is not None
         eps = s.qk_norm.eps if s.qk_norm is not None else 0.0
         window = s.window or 0
         if self.chunk is not None:
@@ -398,6 +419,7 @@ class AttentionMixer:
         proj = self.qkv.partial(x, cheap_sum=True)
         part = proj if proj.dim() == 3 else None
         if (ctx.mode == DECODE and part is not None and hdv == hd and not self.whole_norm and
+                not codes and
                 self.dist_bias is None and not self.keep_first and
                 not self.row_extras and not self.softcap and
                 kernels.attention_decode_fused_supported(self.dtype, hd, rotary_dim)):
@@ -414,7 +436,8 @@ class AttentionMixer:
             if self.value_mix is not None and self.value_mix.source is not None:
                 v_first = ctx.step_values[self.value_mix.source]
             kernels.proj_norm_store(qkv, nh * hd, nkv * hd, nkv * hdv, self.q_norm_weight,
-                                    self.k_norm_weight, eps, ctx.positions, view, ctx,
+                                    self.k_norm_weight, eps, ctx.positions,
+                                    view if not codes else None, ctx,
                                     partial=part, v_first=v_first, v_mix=self.mix_weight)
             if self.value_mix is not None and self.value_mix.source is None:
                 # the values as projected, for the layers that lean on them
@@ -423,9 +446,10 @@ class AttentionMixer:
             if ctx.mode == PREFILL and kernels.attention_prefill_wants_transposed_values(
                     qkv, ctx, nh, nkv, hd, hdv):
                 vt = kernels.prefill_values_scratch(T, ctx.batch, nkv, hdv, qkv.device)
+            pools = (view.k_pool, view.v_pool) if not codes else (None, None)
             kernels.qk_norm_rope_store(
                 qkv, nh, nkv, hd, self.q_norm_weight, self.k_norm_weight, eps, cos, sin,
-                rotary_dim, ctx.positions, view.k_pool, view.v_pool, view.page_table, ctx.slots,
+                rotary_dim, ctx.positions, *pools, view.page_table, ctx.slots,
                 ctx.lens, ctx.seq_index, view.page, view.cap, partial=part, vt=vt,
                 cu_seqlens=ctx.cu_seqlens, max_len=ctx.max_new, value_dim=hdv,
                 q_temp=self.q_temp, bias=self.bias, interleaved=self.interleaved,
@@ -435,6 +459,8 @@ class AttentionMixer:
                                        rotary_dim, ctx.positions, partial=part, value_dim=hdv,
                                        q_temp=self.q_temp, bias=self.bias,
                                        interleaved=self.interleaved)
+        if codes and self.own_kv:
+            self._store_codes(qkv, view, ctx)
         q = qkv[:, :nh * hd]
         out = ctx.new(T, nh * hdv)
         if ctx.mode == PREFILL:
@@ -492,7 +518,9 @@ class AttentionMixer:
             state = ctx.cache.state_view(entry).state
         kernels.conv_rope_store(row, part, qkvg, nh, n_own, hd, hdv, taps, self.conv_w, cos, sin,
                                 rotary_dim, self.out_gate, state, 0, ctx,
-                                view if self.own_kv else None)
+                                view if self.own_kv and view.k_scale is None else None)
+        if self.own_kv and view.k_scale is not None:
+            self._store_codes(qkvg, view, ctx)
         q = qkvg[:, :nh * hd]
         out = ctx.new(T, nh * hdv)
         if ctx.mode == PREFILL:

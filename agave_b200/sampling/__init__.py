@@ -1,3 +1,3 @@
-from .sampler import HISTORY_CAP, Sampler, SamplingParams
+from .sampler import HISTORY_CAP, Sampler, SamplingParams, TokenScore
 
-__all__ = ["HISTORY_CAP", "Sampler", "SamplingParams"]
+__all__ = ["HISTORY_CAP", "Sampler", "SamplingParams", "TokenScore"]

@@ -14,7 +14,7 @@ from __future__ import annotations
 
 import time
 from dataclasses import dataclass
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
@@ -49,6 +49,18 @@ class SamplingParams:
 
     def resolved_seed(self) -> int:
         return self.seed if self.seed is not None else time.time_ns() & 0xFFFFFFFFFFFF
+
+
+@dataclass(frozen=True)
+class TokenScore:
+    """What the model's logits (before penalty and temperature) say of one token: its log-probability
+    and the entropy of its row in nats, its rank (1 = the most likely) and the most likely tokens
+    with theirs."""
+    token: int
+    logprob: float
+    entropy: float
+    rank: int
+    top: Tuple[Tuple[int, float], ...] = ()
 
 
 class Sampler:

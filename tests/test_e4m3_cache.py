@@ -103,3 +103,19 @@ def test_logprobs_refuses(lib):
                      (dict(top=4, V=3), "top"), (dict(top=-1), "top"), (dict(dtype=2), "dtype")):
         rc, msg = call(**kw)
         assert rc < 0 and word in msg, (kw, msg)
+
+
+def test_command_line_options():
+    from agave_b200.cli import _holds_codes, _unsupported, build_parser, main
+    p = build_parser()
+    for argv, codes in (([], False), (["--kv-type", "bf16"], False), (["--kv-type", "e4m3"], True),
+                        (["--kv-type", "FP8"], True), (["--kv-type-k", "f8", "--kv-type-v", "e4m3"], True),
+                        (["--cache-type-k", "fp8", "--cache-type-v", "fp8"], True),
+                        (["--kv-type", "fp8", "--kv-type-k", "fp8"], True)):
+        args = p.parse_args(["m"] + argv)
+        assert _unsupported(args) is None and _holds_codes(args) is codes, argv
+    for argv in (["--kv-type", "e4m3", "--kv-type-v", "bf16"], ["--kv-type-k", "e4m3"], ["--kv-type-v", "e4m3"],
+                 ["--kv-type-k", "e4m3", "--kv-type-v", "bf16"], ["--kv-type", "bf16", "--kv-type-k", "fp8"],
+                 ["--kv-type", "q4_0"], ["--kv-type", "turbo4"]):
+        assert _unsupported(p.parse_args(["m"] + argv)) is not None, argv
+    assert main(["/tmp", "--tokens", "1", "--logprobs", "33"]) == 1
