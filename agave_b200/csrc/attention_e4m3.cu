@@ -24,6 +24,7 @@
 // scale of a page's values is part of the weights, relative to the greatest one so far and times
 // 2^14: a half holds a weight of up to 2^14 and, 11 bits, down to 2^-14.
 #include "e4m3.cuh"
+#include <atomic>
 
 namespace {
 
@@ -43,9 +44,10 @@ struct AttendE4 {
     int B, n_slots, max_pages, n_pages, page, cap, nh, nkv, hd, hdv, window, keep_first;
     float scale, softcap;
     const float *sinks, *dist_bias;
-    int n_dist, q_vec;
+    int n_dist, q_vec, page_bits;
     int row_blocks;                           // blocks of 8 query heads of a kv head
-    float* partial;                           // null: a CTA takes whole rows
+    int cluster;                              // CTAs that share a row where there are no stretches
+    float* partial;                           // null: no stretches
 };
 
 // Head sizes are padded with zeros to DIM = 64, 128 or 256.
@@ -125,22 +127,26 @@ __device__ __forceinline__ Seen seen_by(const AttendE4& a, int b) {
     return s;
 }
 
-// The sequences' tiles on one line.  ``scan``: 8 ints of shared memory.  All threads of a CTA of
-// AE_THREADS take part and get the result.
-__device__ __forceinline__ int all_tiles(const AttendE4& a, int* scan) {
+// The sequences' tiles on one line.  ``scan``: 2 ints of shared memory, ``scratch``: 32 floats of it.
+// All THREADS of a CTA take part and get the result.
+template <int THREADS>
+__device__ __forceinline__ int all_tiles(const AttendE4& a, int* scan, float* scratch) {
     int n = 0;
-    for (int b = threadIdx.x; b < a.B; b += AE_THREADS) n += seen_by(a, b).tiles;
+    for (int b = threadIdx.x; b < a.B; b += THREADS) n += seen_by(a, b).tiles;
     n = __reduce_add_sync(0xffffffffu, n);
+    int* sums = reinterpret_cast<int*>(scratch);
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) scan[threadIdx.x >> 5] = n;
+    if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = n;
     __syncthreads();
-    return scan[0] + scan[1] + scan[2] + scan[3];
+    return __reduce_add_sync(0xffffffffu, (threadIdx.x & 31) < THREADS / 32 ? sums[threadIdx.x & 31] : 0);
 }
 // The sequence that tile y of the line belongs to, and the tiles before it.
-__device__ __forceinline__ void find_tile(const AttendE4& a, int y, int* scan, int& seq, int& before) {
+template <int THREADS>
+__device__ __forceinline__ void find_tile(const AttendE4& a, int y, int* scan, float* scratch, int& seq, int& before) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int* sums = reinterpret_cast<int*>(scratch);
     int done = 0;
-    for (int base = 0; base < a.B; base += AE_THREADS) {
+    for (int base = 0; base < a.B; base += THREADS) {
         const int b = base + threadIdx.x;
         const int n = b < a.B ? seen_by(a, b).tiles : 0;
         int upto = n;
@@ -150,26 +156,94 @@ __device__ __forceinline__ void find_tile(const AttendE4& a, int y, int* scan, i
             if (lane >= o) upto += t;
         }
         __syncthreads();
-        if (lane == 31) scan[warp] = upto;
+        if (lane == 31) sums[warp] = upto;
         __syncthreads();
         int total = 0;
 #pragma unroll
-        for (int w = 0; w < AE_WARPS; ++w) {
-            if (w < warp) upto += scan[w];
-            total += scan[w];
+        for (int w = 0; w < THREADS / 32; ++w) {
+            if (w < warp) upto += sums[w];
+            total += sums[w];
         }
         if (y < done + total) {
-            if (y >= done + upto - n && y < done + upto) { scan[4] = b; scan[5] = done + upto - n; }
+            if (y >= done + upto - n && y < done + upto) { scan[0] = b; scan[1] = done + upto - n; }
             break;
         }
         done += total;
     }
     __syncthreads();
-    seq = scan[4];
-    before = scan[5];
+    seq = scan[0];
+    before = scan[1];
 }
 __device__ __forceinline__ long long stretch_start(long long units, int cta, int ctas) {
     return units * cta / ctas;
+}
+
+__device__ __forceinline__ void cluster_meet() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float peer_f32(const void* mine, int rank) {
+    unsigned at;
+    float v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((unsigned)__cvta_generic_to_shared(mine)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+// The CTAs of a cluster join their results for a row: each brings its warps' sums together in its
+// own shared memory, and writes its share of the output from everybody's.
+template <typename T, int DIM>
+__device__ __forceinline__ void share_row(const AttendE4& a, float* red, float (*stat)[AE_HEADS][2], int b, int h0,
+                                          int heads) {
+    using S = Tile<DIM>;
+    __shared__ float ml[AE_HEADS][2];
+    __shared__ float weight[AE_HEADS][16];
+    const int tid = threadIdx.x, C = a.cluster, rank = blockIdx.x % C;
+    for (int i = tid; i < heads * DIM; i += AE_THREADS) {
+        float* at = red + i / DIM * S::RED + i % DIM;
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < AE_WARPS; ++w) v += at[w * AE_HEADS * S::RED];
+        *at = v;
+    }
+    if (tid < AE_HEADS) {
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < AE_WARPS; ++w) M = fmaxf(M, stat[w][tid][0]);
+#pragma unroll
+        for (int w = 0; w < AE_WARPS; ++w) L += stat[w][tid][1] * (M == -INFINITY ? 1.f : ex2(stat[w][tid][0] - M));
+        ml[tid][0] = M;
+        ml[tid][1] = L;
+    }
+    cluster_meet();
+    // a thread a (head, CTA): what the CTA's sums are multiplied by
+    static_assert(AE_THREADS == 16 * AE_HEADS, "16 CTAs at most for each of the heads");
+    {
+        const int h = tid >> 4, r = tid & 15;
+        float m = -INFINITY, l = 0.f;
+        if (r < C) {
+            m = peer_f32(&ml[h][0], r);
+            l = peer_f32(&ml[h][1], r);
+        }
+        float M = m;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        const float sink = a.sinks && h < heads ? a.sinks[h0 + h] * 1.4426950408889634f : -INFINITY;
+        M = fmaxf(M, sink);
+        const float w = M == -INFINITY ? 1.f : ex2(m - M);
+        float L = l * w;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+        if (sink != -INFINITY) L += ex2(sink - M);
+        weight[h][r] = L == 0.f ? 0.f : w / L;
+    }
+    __syncthreads();
+    T* out = (T*)a.out + ((size_t)b * a.nh + h0) * a.hdv;
+    for (int i = rank * AE_THREADS + tid; i < heads * a.hdv; i += C * AE_THREADS) {
+        const int h = i / a.hdv, d = i % a.hdv;
+        float v = 0.f;
+        for (int r = 0; r < C; ++r) v += peer_f32(red + h * S::RED + d, r) * weight[h][r];
+        out[i] = from_f32<T>(v);
+    }
+    cluster_meet();                            // (a CTA's memory stays until its peers have read it)
 }
 
 // ---------------------------------------------------------------- the walk over the keys
@@ -180,7 +254,8 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
     constexpr int NQ = DIM / 64, NT = DIM / 16;
     constexpr int VB = DIM >= 128 ? 16 : 8, NV = DIM / (8 * VB); // bytes of values at a time, times
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ int scan[8];
+    __shared__ int scan[2];
+    __shared__ float scratch[32];
     __shared__ float stat[AE_WARPS][AE_HEADS][2];
     __shared__ float meta[AE_WARPS][S::STAGES][4];               // scales of keys and values, page is there
     pdl_wait();
@@ -195,77 +270,114 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
     long long left;                                              // units still to do
     int tile;
     if (a.partial) {
-        const int total = all_tiles(a, scan);
+        const int total = all_tiles<AE_THREADS>(a, scan, scratch);
         const long long units = (long long)total * R;
         const long long x0 = stretch_start(units, blockIdx.x, gridDim.x);
         left = stretch_start(units, blockIdx.x + 1, gridDim.x) - x0;
         if (left == 0) return;
-        find_tile(a, (int)(x0 / R), scan, b, before);
+        find_tile<AE_THREADS>(a, (int)(x0 / R), scan, scratch, b, before);
         const int n = seen_by(a, b).tiles;
         const long long in = x0 - (long long)before * R;
         row = (int)(in / n);
         tile = (int)(in - (long long)row * n);
     } else {
-        b = blockIdx.x / R;
-        row = blockIdx.x % R;
-        tile = 0;
-        left = seen_by(a, b).tiles;
+        const int unit = blockIdx.x / a.cluster, part = blockIdx.x % a.cluster;
+        b = unit / R;
+        row = unit % R;
+        const int n = seen_by(a, b).tiles;
+        tile = n * part / a.cluster;
+        left = n * (part + 1) / a.cluster - tile;
     }
+    const bool shared_row = !a.partial && a.cluster > 1;
     int segment = 0;
-    while (left > 0) {
+    while (left > 0 || (shared_row && segment == 0)) {
         const Seen s = seen_by(a, b);
         const int g = row / a.row_blocks, h0 = g * group + row % a.row_blocks * AE_HEADS;
         const int heads = min(AE_HEADS, (g + 1) * group - h0);
         const int n = (int)min((long long)(s.tiles - tile), left);   // tiles of this segment
         const bool whole = n == s.tiles;
         if (s.slot < 0) {
+            if (!shared_row || left > 0) {
             T* out = (T*)a.out + ((size_t)b * a.nh + h0) * a.hdv;
             for (int i = tid; i < heads * a.hdv; i += AE_THREADS) out[i] = from_f32<T>(0.f);
+            }
         } else {
             const int* table = a.table + (size_t)s.slot * a.max_pages;
             const size_t krow = (size_t)a.nkv * a.hd, vrow = (size_t)a.nkv * a.hdv;
-            // position of this warp's part of tile i of the segment, and the page it lies in
-            auto place = [&](int i) {
-                const int t = tile + i;
-                return (t < s.kept_tiles ? t : s.first_tile + t - s.kept_tiles) * AE_TILE + warp * 16;
+            // The tiles are visited in order, this warp's 16 positions of each: their first position and
+            // its row of the ring, one step after the other (a division only where the kept tiles end).
+            struct Place {
+                int t, j, row;
             };
-            auto page_of = [&](int i) {
-                if (i >= n) return -1;
-                const int j = place(i);
-                return j <= s.p ? table[j % a.cap / a.page] : -1;
+            auto start = [&](int t) {
+                Place at;
+                at.t = t;
+                at.j = (t < s.kept_tiles ? t : s.first_tile + t - s.kept_tiles) * AE_TILE + warp * 16;
+                at.row = at.j % a.cap;
+                return at;
+            };
+            auto advance = [&](Place& at) {
+                if (++at.t == s.kept_tiles) {
+                    at = start(at.t);
+                } else {
+                    at.j += AE_TILE;
+                    at.row += AE_TILE;
+                    while (at.row >= a.cap) at.row -= a.cap;
+                }
+            };
+            const int t_end = tile + n;
+            auto page_of = [&](const Place& at) {
+                return at.t < t_end && at.j <= s.p ? table[at.row >> a.page_bits] : -1;
             };
             constexpr int LPR = DIM / 16, RPI = 32 / LPR;        // lanes a row, rows an instruction
             const int crow = lane / LPR, ccol = lane % LPR * 16;
-            auto issue = [&](int i, int pg, int stage) {
-                if (i < n) {
-                    const int j0 = place(i);
+            const unsigned copy_at = mine_at + crow * S::KS + ccol, copy_vat = mine_at + 16 * S::KS + crow * S::VS + ccol;
+            const int k_bytes = ccol < a.hd ? 16 : 0, v_bytes = ccol < a.hdv ? 16 : 0;
+            const unsigned char* k_from = a.k_pool + (size_t)crow * krow + (size_t)g * a.hd + (k_bytes ? ccol : 0);
+            const unsigned char* v_from = a.v_pool + (size_t)crow * vrow + (size_t)g * a.hdv + (v_bytes ? ccol : 0);
+            auto issue = [&](const Place& at, int pg, int stage) {
+                if (at.t < t_end) {
                     const bool there = pg >= 0 && pg < a.n_pages;
                     const int page = there ? pg : 0;
-                    const size_t at = (size_t)page * a.page + j0 % a.cap % a.page;
-                    const unsigned char* k = a.k_pool + at * krow + (size_t)g * a.hd;
-                    const unsigned char* v = a.v_pool + at * vrow + (size_t)g * a.hdv;
-                    const unsigned ks = mine_at + stage * S::STAGE, vs = ks + 16 * S::KS;
-                    const bool all = there && j0 >= s.first && j0 + 15 <= s.p;
+                    const size_t from = ((size_t)page << a.page_bits) + (at.row & (a.page - 1));
+                    const unsigned char *k = k_from + from * krow, *v = v_from + from * vrow;
+                    const unsigned ks = copy_at + stage * S::STAGE, vs = copy_vat + stage * S::STAGE;
+                    if (there && at.j >= s.first && at.j + 15 <= s.p) {
 #pragma unroll
-                    for (int q = 0; q < 16 / RPI; ++q) {
-                        const int rr = q * RPI + crow, j = j0 + rr;
-                        const bool ok = all || (there && j <= s.p && (j >= s.first || j < s.kept));
-                        const int kb = ok && ccol < a.hd ? 16 : 0, vb = ok && ccol < a.hdv ? 16 : 0;
-                        copy16(ks + rr * S::KS + ccol, kb ? k + rr * krow + ccol : a.k_pool, kb);
-                        copy16(vs + rr * S::VS + ccol, vb ? v + rr * vrow + ccol : a.v_pool, vb);
+                        for (int q = 0; q < 16 / RPI; ++q) {
+                            copy16(ks + q * RPI * S::KS, k, k_bytes);
+                            copy16(vs + q * RPI * S::VS, v, v_bytes);
+                            k += RPI * krow;
+                            v += RPI * vrow;
+                        }
+                    } else {
+                        // (rows that are not seen become zeros: whatever their codes are, they add nothing)
+#pragma unroll
+                        for (int q = 0; q < 16 / RPI; ++q) {
+                            const int j = at.j + q * RPI + crow;
+                            const bool ok = there && j <= s.p && (j >= s.first || j < s.kept);
+                            copy16(ks + q * RPI * S::KS, k, ok ? k_bytes : 0);
+                            copy16(vs + q * RPI * S::VS, v, ok ? v_bytes : 0);
+                            k += RPI * krow;
+                            v += RPI * vrow;
+                        }
                     }
                     if (lane == 0) {
-                        const unsigned at = (unsigned)__cvta_generic_to_shared(meta[warp][stage]);
-                        copy4(at, a.k_scale + (size_t)page * a.nkv + g);
-                        copy4(at + 4, a.v_scale + (size_t)page * a.nkv + g);
+                        const unsigned to = (unsigned)__cvta_generic_to_shared(meta[warp][stage]);
+                        copy4(to, a.k_scale + (size_t)page * a.nkv + g);
+                        copy4(to + 4, a.v_scale + (size_t)page * a.nkv + g);
                         meta[warp][stage][2] = there ? 1.f : 0.f;
                     }
                 }
                 copies_commit();
             };
+            Place now = start(tile), next = now;
 #pragma unroll
-            for (int i = 0; i < S::STAGES - 1; ++i) issue(i, page_of(i), i);
-            int next_page = page_of(S::STAGES - 1);
+            for (int i = 0; i < S::STAGES - 1; ++i) {
+                issue(next, page_of(next), i);
+                advance(next);
+            }
+            int next_page = page_of(next);
 
             // the queries: head r, dimensions i * 64 + c * 16 .. + 15
             unsigned qh[NQ][8], ql[SPLIT ? NQ : 1][8];
@@ -316,24 +428,27 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
                     }
             }
             // this thread's columns of the scores and sums: heads 2 c and 2 c + 1
-            const float f0 = __shfl_sync(0xffffffffu, qf, 8 * c) * a.scale;
-            const float f1 = __shfl_sync(0xffffffffu, qf, 8 * c + 4) * a.scale;
+            constexpr float LOG2E = 1.4426950408889634f;
+            const bool extras = a.softcap > 0.f || a.dist_bias;
+            const float unit = extras ? a.scale : a.scale * LOG2E;
+            const float f0 = __shfl_sync(0xffffffffu, qf, 8 * c) * unit;
+            const float f1 = __shfl_sync(0xffffffffu, qf, 8 * c + 4) * unit;
             const float* bias = a.dist_bias ? a.dist_bias + (size_t)min(h0 + 2 * c, a.nh - 1) * a.n_dist : nullptr;
             const float* bias1 = a.dist_bias ? a.dist_bias + (size_t)min(h0 + 2 * c + 1, a.nh - 1) * a.n_dist : nullptr;
-            constexpr float LOG2E = 1.4426950408889634f;
 
             float o[NT][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, vref = 0.f, vlast = -1.f, vf = 0.f;
 #pragma unroll
             for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
 
             int stage = 0;
-            for (int i = 0; i < n; ++i) {
+            for (; now.t < t_end; advance(now)) {
                 const int ahead = stage == 0 ? S::STAGES - 1 : stage - 1;
-                issue(i + S::STAGES - 1, next_page, ahead);
-                next_page = page_of(i + S::STAGES);
+                issue(next, next_page, ahead);
+                advance(next);
+                next_page = page_of(next);
                 copies_wait<S::STAGES - 1>();
                 __syncwarp();
-                const int j0 = place(i);
+                const int j0 = now.j;
                 if (j0 <= s.p && meta[warp][stage][2] != 0.f) {
                     const unsigned char* K = mine + stage * S::STAGE;
                     const unsigned char* V = K + 16 * S::KS;
@@ -347,24 +462,37 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
                         const unsigned wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
                         for (int f = 0; f < 4; ++f) {
-                            const unsigned a0 = e4m3_to_half2(wa[f]), a2 = e4m3_to_half2(wa[f] >> 16);
-                            const unsigned a1 = e4m3_to_half2(wb[f]), a3 = e4m3_to_half2(wb[f] >> 16);
+                            unsigned a0, a1, a2, a3;
+                            e4m3_word(wa[f], a0, a2);
+                            e4m3_word(wb[f], a1, a3);
                             mma16816(x[f & 1], a0, a1, a2, a3, qh[q][2 * f], qh[q][2 * f + 1]);
                             if (SPLIT) mma16816(y[f & 1], a0, a1, a2, a3, ql[q][2 * f], ql[q][2 * f + 1]);
                         }
                     }
                     // scores of positions j0 + r, j0 + r + 8 in units of ln 2
                     float p[4];
+                    const float g0 = ks * f0, g1 = ks * f1;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        float v = x[0][e] + x[1][e];
-                        if (SPLIT) v += y[0][e] + y[1][e];
-                        const int j = j0 + r + (e >> 1) * 8;
-                        v *= ks * (e & 1 ? f1 : f0);
-                        if (a.softcap > 0.f) v = soft_capped(v, a.softcap);
-                        if (a.dist_bias) v += (e & 1 ? bias1 : bias)[min(max(s.p - j, 0), a.n_dist - 1)];
-                        const bool ok = j <= s.p && (j >= s.first || j < s.kept);
-                        p[e] = ok ? v * LOG2E : -INFINITY;
+                        p[e] = x[0][e] + x[1][e];
+                        if (SPLIT) p[e] += y[0][e] + y[1][e];
+                        p[e] *= e & 1 ? g1 : g0;
+                    }
+                    if (extras) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int j = j0 + r + (e >> 1) * 8;
+                            if (a.softcap > 0.f) p[e] = soft_capped(p[e], a.softcap);
+                            if (a.dist_bias) p[e] += (e & 1 ? bias1 : bias)[min(max(s.p - j, 0), a.n_dist - 1)];
+                            p[e] *= LOG2E;
+                        }
+                    }
+                    if (j0 < s.first || j0 + 15 > s.p) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int j = j0 + r + (e >> 1) * 8;
+                            if (j > s.p || (j < s.first && j >= s.kept)) p[e] = -INFINITY;
+                        }
                     }
                     float t0 = fmaxf(p[0], p[2]), t1 = fmaxf(p[1], p[3]);
 #pragma unroll
@@ -435,14 +563,16 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
                             const unsigned ha = __byte_perm(w[2][f], w[3][f], 0x5140), hb = __byte_perm(w[2][f], w[3][f], 0x7362);
                             const int t = q * (VB / 2) + 2 * f;
                             {
-                                const unsigned a0 = e4m3_to_half2(la), a1 = e4m3_to_half2(la >> 16);
-                                const unsigned a2 = e4m3_to_half2(ha), a3 = e4m3_to_half2(ha >> 16);
+                                unsigned a0, a1, a2, a3;
+                                e4m3_word(la, a0, a1);
+                                e4m3_word(ha, a2, a3);
                                 mma16816(o[t], a0, a1, a2, a3, b0, b1);
                                 if (SPLIT) mma16816(o[t], a0, a1, a2, a3, c0, c1);
                             }
                             {
-                                const unsigned a0 = e4m3_to_half2(lb), a1 = e4m3_to_half2(lb >> 16);
-                                const unsigned a2 = e4m3_to_half2(hb), a3 = e4m3_to_half2(hb >> 16);
+                                unsigned a0, a1, a2, a3;
+                                e4m3_word(lb, a0, a1);
+                                e4m3_word(hb, a2, a3);
                                 mma16816(o[t + 1], a0, a1, a2, a3, b0, b1);
                                 if (SPLIT) mma16816(o[t + 1], a0, a1, a2, a3, c0, c1);
                             }
@@ -491,6 +621,10 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
             }
             __syncthreads();
             float* part = a.partial ? a.partial + (size_t)(2 * blockIdx.x + (segment > 0)) * S::PART : nullptr;
+            if (shared_row) {
+                share_row<T, DIM>(a, red, stat, b, h0, heads);
+                return;
+            }
             for (int i = tid; i < heads * DIM; i += AE_THREADS) {
                 const int h = i / DIM, d = i % DIM;
                 if (d >= a.hdv) continue;
@@ -534,63 +668,88 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
 
 // ---------------------------------------------------------------- rows of several CTAs
 // CTA (i, h) joins, for head h of 8, the row inside which the stretch of CTA i + 1 begins, if it is
-// the first to begin there.
+// the first to begin there.  First the partial results' weights, a thread each, then the sums:
+// DIM / 4 threads take a partial result, the CTA 8 to 32 of them at a time.
+constexpr int AE_JOIN_THREADS = 512;
+constexpr int AE_MAX_CTAS = 1024;
 template <typename T, int DIM>
-__global__ void __launch_bounds__(AE_THREADS) join_e4m3_kernel(const AttendE4 a, int ctas) {
+__global__ void __launch_bounds__(AE_JOIN_THREADS) join_e4m3_kernel(const AttendE4 a, int ctas) {
     using S = Tile<DIM>;
-    __shared__ int scan[8];
+    __shared__ int scan[2];
+    __shared__ float weight[AE_MAX_CTAS];
+    __shared__ int slot[AE_MAX_CTAS];
+    __shared__ float scratch[32];
+    __shared__ float4 sums[AE_JOIN_THREADS];
     pdl_wait();
     pdl_launch_next();
     const int R = a.nkv * a.row_blocks, group = a.nh / a.nkv, head = blockIdx.y, tid = threadIdx.x;
-    const int total = all_tiles(a, scan);
+    const int total = all_tiles<AE_JOIN_THREADS>(a, scan, scratch);
     const long long units = (long long)total * R;
     const int i = blockIdx.x + 1;
     const long long x = stretch_start(units, i, ctas);
     if (x >= units) return;
     int b, before;
-    find_tile(a, (int)(x / R), scan, b, before);
+    find_tile<AE_JOIN_THREADS>(a, (int)(x / R), scan, scratch, b, before);
     const int n = seen_by(a, b).tiles;
     const int row = (int)((x - (long long)before * R) / n);
     const long long begin = (long long)before * R + (long long)row * n, end = begin + n;
     if (x == begin || stretch_start(units, i - 1, ctas) > begin) return;      // not inside, not the first
     const int g = row / a.row_blocks, h0 = g * group + row % a.row_blocks * AE_HEADS;
     if (h0 + head >= (g + 1) * group) return;
-    constexpr int PER = (DIM + AE_THREADS - 1) / AE_THREADS;
-    float v[PER] = {}, M = -INFINITY, L = 0.f;
-    for (int j = i - 1; j < ctas; ++j) {
-        const long long from = stretch_start(units, j, ctas);
-        if (from >= end) break;
-        if (stretch_start(units, j + 1, ctas) == from) continue;              // no work
-        const float* part = a.partial + (size_t)(2 * j + (from < begin)) * S::PART;
-        const float m = part[AE_HEADS * DIM + 2 * head], l = part[AE_HEADS * DIM + 2 * head + 1];
-        const float N = fmaxf(M, m);
-        const float f0 = N == -INFINITY ? 1.f : ex2(M - N), f1 = N == -INFINITY ? 1.f : ex2(m - N);
-        M = N;
-        L = L * f0 + l * f1;
-#pragma unroll
-        for (int e = 0; e < PER; ++e) {
-            const int d = tid + e * AE_THREADS;
-            if (d < a.hdv) v[e] = v[e] * f0 + part[head * DIM + d] * f1;
+    // the CTAs i - 1 .. last have a part of the row (but for those whose stretch is empty)
+    const int last = (int)((end * ctas - 1) / units), parts = last - i + 2;
+    float M = -INFINITY;
+    for (int j = tid; j < parts; j += AE_JOIN_THREADS) {
+        const int cta = i - 1 + j;
+        const long long from = stretch_start(units, cta, ctas);
+        const int at = from == stretch_start(units, cta + 1, ctas) ? -1 : 2 * cta + (from < begin);
+        slot[j] = at;
+        weight[j] = at < 0 ? -INFINITY : a.partial[(size_t)at * S::PART + AE_HEADS * DIM + 2 * head];
+        M = fmaxf(M, weight[j]);
+    }
+    M = block_max(M, scratch);
+    const float sink = a.sinks ? a.sinks[h0 + head] * 1.4426950408889634f : -INFINITY;
+    M = fmaxf(M, sink);
+    float L = 0.f;
+    for (int j = tid; j < parts; j += AE_JOIN_THREADS) {
+        const float w = M == -INFINITY ? 1.f : ex2(weight[j] - M);
+        weight[j] = w;
+        if (slot[j] >= 0) L += w * a.partial[(size_t)slot[j] * S::PART + AE_HEADS * DIM + 2 * head + 1];
+    }
+    L = block_sum(L, scratch);                 // (with barriers: the weights are there)
+    if (sink != -INFINITY) L += ex2(sink - M);
+    constexpr int LANES = DIM / 4, GROUPS = AE_JOIN_THREADS / LANES;
+    const int d = tid % LANES * 4;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (d < a.hdv) {
+#pragma unroll 4
+        for (int j = tid / LANES; j < parts; j += GROUPS) {
+            const int at = slot[j];
+            if (at < 0) continue;
+            const float4 u = *reinterpret_cast<const float4*>(a.partial + (size_t)at * S::PART + head * DIM + d);
+            const float w = weight[j];
+            v.x = fmaf(u.x, w, v.x);
+            v.y = fmaf(u.y, w, v.y);
+            v.z = fmaf(u.z, w, v.z);
+            v.w = fmaf(u.w, w, v.w);
         }
     }
-    if (a.sinks) {
-        const float sink = a.sinks[h0 + head] * 1.4426950408889634f, N = fmaxf(M, sink);
-        const float f = M == -INFINITY ? 0.f : ex2(M - N);
-        L = L * f + ex2(sink - N);
-#pragma unroll
-        for (int e = 0; e < PER; ++e) v[e] *= f;
-    }
+    sums[tid] = v;
+    __syncthreads();
+    const float* flat = reinterpret_cast<const float*>(sums);
     T* out = (T*)a.out + ((size_t)b * a.nh + h0 + head) * a.hdv;
+    for (int e = tid; e < a.hdv; e += AE_JOIN_THREADS) {
+        float o = 0.f;
 #pragma unroll
-    for (int e = 0; e < PER; ++e) {
-        const int d = tid + e * AE_THREADS;
-        if (d < a.hdv) out[d] = from_f32<T>(L == 0.f ? 0.f : v[e] / L);
+        for (int q = 0; q < GROUPS; ++q) o += flat[q * DIM + e];
+        out[e] = from_f32<T>(L == 0.f ? 0.f : o / L);
     }
 }
 
 struct Plan {
     int dim, ctas;             // padded head size; CTAs of the launch
     bool split;                // stretches of an equal number of tiles, joined afterwards
+    int cluster;               // else: CTAs that share a row
 };
 int sm_count() {
     static int n = 0;
@@ -609,19 +768,33 @@ Plan plan_of(int B, int nh, int nkv, int hd, int hdv, int max_keys) {
     const long long rows = (long long)B * nkv * ((nh / nkv + AE_HEADS - 1) / AE_HEADS);
     const long long tiles = (max_keys + AE_TILE - 1) / AE_TILE + 1;
     const int resident = sm_count() * (p.dim == 256 ? Tile<256>::CTAS : p.dim == 128 ? Tile<128>::CTAS : Tile<64>::CTAS);
-    p.split = tiles > 8;
-    p.ctas = (int)(!p.split || rows * tiles < resident ? (p.split ? rows * tiles : rows) : resident);
+    // A row is the work of a cluster's CTAs where that leaves each a few tiles: one launch, and the
+    // join goes through shared memory.  Else stretches: CTAs for every row there is room for.
+    p.cluster = 1;
+    while (p.cluster < 16 && p.cluster < tiles && rows * p.cluster * 2 <= resident) p.cluster *= 2;
+    p.split = tiles > 8 * p.cluster;
+    if (!p.split) p.ctas = (int)(rows * p.cluster);
+    else p.ctas = (int)(rows * tiles < resident ? rows * tiles : resident);
+    if (p.split && p.ctas > AE_MAX_CTAS) p.ctas = AE_MAX_CTAS;
     return p;
 }
 template <typename T, int DIM>
 int launch(const AttendE4& a, const Plan& p, cudaStream_t stream) {
-    AGV_CUDA_OK(cudaFuncSetAttribute(attend_e4m3_kernel<T, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     Tile<DIM>::SMEM));
-    agv_launch(attend_e4m3_kernel<T, DIM>, p.ctas, AE_THREADS, Tile<DIM>::SMEM, stream, a);
+    static std::atomic<unsigned long long> ready{0};             // devices on which the kernel has been set up
+    int dev = 0;
+    AGV_CUDA_OK(cudaGetDevice(&dev));
+    if (!(ready.load() >> (dev & 63) & 1)) {
+        AGV_CUDA_OK(cudaFuncSetAttribute(attend_e4m3_kernel<T, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         Tile<DIM>::SMEM));
+        AGV_CUDA_OK(cudaFuncSetAttribute(attend_e4m3_kernel<T, DIM>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        ready.fetch_or(1ull << (dev & 63));
+    }
+    agv_launch_cluster(attend_e4m3_kernel<T, DIM>, p.ctas, AE_THREADS, Tile<DIM>::SMEM, stream,
+                       dim3(p.split ? 1 : p.cluster), a);
     AGV_LAUNCH_OK("attend_e4m3_kernel");
     if (p.split && p.ctas > 1) {
         const int heads = a.nh / a.nkv < AE_HEADS ? a.nh / a.nkv : AE_HEADS;
-        agv_launch(join_e4m3_kernel<T, DIM>, dim3(p.ctas - 1, heads), AE_THREADS, 0, stream, a, p.ctas);
+        agv_launch(join_e4m3_kernel<T, DIM>, dim3(p.ctas - 1, heads), AE_JOIN_THREADS, 0, stream, a, p.ctas);
         AGV_LAUNCH_OK("join_e4m3_kernel");
     }
     return 0;
@@ -660,20 +833,22 @@ AGV_API int agv_attention_decode_e4m3(const void* q, long long ldq, void* out, i
                 "attention_decode_e4m3: bad sizes (%d query heads over %d)", nh, nkv);
     AGV_REQUIRE(hd > 0 && hd % 16 == 0 && hd <= AE_MAX_DIM && hdv > 0 && hdv % 16 == 0 && hdv <= AE_MAX_DIM,
                 "attention_decode_e4m3: head sizes %d and %d must be multiples of 16 up to %d", hd, hdv, AE_MAX_DIM);
-    AGV_REQUIRE(page > 0 && page % 16 == 0 && cap > 0 && cap % page == 0 && cap / page <= max_pages,
+    AGV_REQUIRE(page >= 16 && (page & (page - 1)) == 0 && cap > 0 && cap % page == 0 && cap / page <= max_pages,
                 "attention_decode_e4m3: bad cache geometry (page %d, cap %d, table of %d)", page, cap, max_pages);
     AGV_REQUIRE(dtype == AGV_F32 || dtype == AGV_BF16, "attention_decode_e4m3: bad dtype");
     AGV_REQUIRE(agv_aligned(k_pool, 16) && agv_aligned(v_pool, 16), "attention_decode_e4m3: unaligned pool");
     AGV_REQUIRE(keep_first >= 0 && softcap >= 0.f && (!dist_bias || n_dist > 0), "attention_decode_e4m3: bad options");
     if (B == 0) return 0;
     const Plan plan = plan_of(B, nh, nkv, hd, hdv, max_keys);
-    AGV_REQUIRE(!plan.split || (partial && partial_floats >= agv_attention_decode_e4m3_scratch(B, nh, nkv, hd, hdv, max_keys)),
+    AGV_REQUIRE(!plan.split || (partial && agv_aligned(partial, 16) && partial_floats >= agv_attention_decode_e4m3_scratch(B, nh, nkv, hd, hdv, max_keys)),
                 "attention_decode_e4m3: %lld floats of scratch are too few", partial_floats);
     const size_t esz = dtype == AGV_F32 ? 4 : 2;
+    int page_bits = 0;
+    while (1 << page_bits < page) ++page_bits;
     const int q_vec = agv_aligned(q, 16) && (size_t)ldq * esz % 16 == 0;
     AttendE4 a{q, ldq, out, (const unsigned char*)k_pool, (const unsigned char*)v_pool, k_scale, v_scale,
                table, slots, positions, B, n_slots, max_pages, n_pages, page, cap, nh, nkv, hd, hdv,
                window, window ? keep_first : 0, scale, softcap, sinks, dist_bias, n_dist, q_vec,
-               (nh / nkv + AE_HEADS - 1) / AE_HEADS, plan.split ? partial : nullptr};
+               page_bits, (nh / nkv + AE_HEADS - 1) / AE_HEADS, plan.cluster, plan.split ? partial : nullptr};
     return dtype == AGV_F32 ? launch_dim<float>(a, plan, stream) : launch_dim<__nv_bfloat16>(a, plan, stream);
 }

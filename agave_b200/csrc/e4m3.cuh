@@ -48,3 +48,8 @@ __device__ __forceinline__ float2 e4m3_to_float2(unsigned codes) {
         : "=f"(lo), "=f"(hi) : "r"(h));
     return make_float2(lo, hi);
 }
+// Four codes as two pairs of half floats.
+__device__ __forceinline__ void e4m3_word(unsigned codes, unsigned& lo, unsigned& hi) {
+    asm("{.reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;}"
+        : "=r"(lo), "=r"(hi) : "r"(codes));
+}

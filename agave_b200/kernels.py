@@ -34,6 +34,16 @@ def _act(activation, w2):
         raise KernelError("the clamped activation goes with a gated pair and a positive limit")
     return ACT[kind], ctypes.c_float(alpha), ctypes.c_float(limit)
 
+# Arguments of functions that are called with plain numbers and addresses (which costs a fraction of
+# what wrapping each does): p address, i int, l long long, f float.
+_KINDS = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
+_PROTOTYPES = {
+    "agv_cache_store_e4m3": (ctypes.c_int, "plpl" "ipppiiiiii" "ppppp" "iiiii" "p"),
+    "agv_attention_decode_e4m3_scratch": (ctypes.c_longlong, "iiiiii"),
+    "agv_attention_decode_e4m3": (ctypes.c_int, "plpi" "ppppp" "iiiii" "pp" "iiiii" "fii" "ppifi" "pl" "p"),
+    "agv_token_logprobs": (ctypes.c_int, "pli" "ii" "pi" "ppppp" "p"),
+}
+
 _lib = None
 _lock = threading.Lock()
 
@@ -55,7 +65,9 @@ def library() -> ctypes.CDLL:
                     raise KernelError(f"the CUDA library {path} could not be loaded: {e}") from None
                 lib.agv_last_error.restype = ctypes.c_char_p
                 lib.agv_attention_prefill_tc_vt_cols.restype = ctypes.c_longlong
-                lib.agv_attention_decode_e4m3_scratch.restype = ctypes.c_longlong
+                for name, (result, kinds) in _PROTOTYPES.items():
+                    f = getattr(lib, name)
+                    f.restype, f.argtypes = result, [_KINDS[k] for k in kinds]
                 if os.environ.get("AGAVE_B200_DEPENDENT_LAUNCH", "1") == "0":
                     # kernels then start only after the one before has ended, which
                     # makes per-kernel durations in a profiler additive
@@ -145,9 +157,18 @@ def _on_current_device(*tensors) -> None:
     """All given tensors lie on the CUDA device that is current: the launch goes to its stream."""
     dev = _raw_device() if _raw_device is not None else torch.cuda.current_device()
     for t in tensors:
-        if t is not None and not (t.is_cuda and t.get_device() == dev):
+        if t is not None and t.get_device() != dev:              # (-1 off CUDA)
             raise KernelError(f"a tensor on {t.device} was handed to a kernel; the current CUDA "
                               f"device is cuda:{dev}")
+
+
+def _stream_handle() -> int:
+    """The current stream as a number; counts a launch, as ``_stream`` does."""
+    global _launches
+    _launches += 1
+    if _raw_stream is not None and _raw_device is not None:
+        return _raw_stream(_raw_device())
+    return torch.cuda.current_stream().cuda_stream
 
 
 def device_arch() -> int:
@@ -2032,20 +2053,23 @@ def e4m3_head_supported(head_dim: int, value_dim: int = 0) -> bool:
 
 def _e4m3_view(view, n_kv_heads: int, head_dim: int, value_dim: int, what: str):
     """Checks a cache entry's pools, scales and table; (slots of the table, its width, pages)."""
-    k, v, table = view.k_pool, view.v_pool, view.page_table
+    k, v, ks, vs, table = view.k_pool, view.v_pool, view.k_scale, view.v_scale, view.page_table
     _require(k.dtype == E4M3 and v.dtype == E4M3, f"{what}: the pools must hold float8_e4m3fn codes")
-    _require(k.dim() == 4 and v.dim() == 4 and k.shape[1:] == (view.page, n_kv_heads, head_dim) and
-             v.shape[1:] == (view.page, n_kv_heads, value_dim) and v.shape[0] == k.shape[0],
-             f"{what}: pools {tuple(k.shape)} and {tuple(v.shape)} are not [pages, {view.page}, "
-             f"{n_kv_heads}, head size]")
-    _require(k.is_contiguous() and v.is_contiguous() and table.is_contiguous() and
-             view.k_scale.is_contiguous() and view.v_scale.is_contiguous(),
-             f"{what}: pools, scales and page table must be contiguous")
-    for s in (view.k_scale, view.v_scale):
-        _require(s.dtype == torch.float32 and s.shape == (k.shape[0], n_kv_heads),
-                 f"{what}: scales must be float32 [{k.shape[0]}, {n_kv_heads}]")
+    shape = k.shape
+    pages = shape[0]
+    if shape != (pages, view.page, n_kv_heads, head_dim) or \
+            v.shape != (pages, view.page, n_kv_heads, value_dim):
+        raise KernelError(f"{what}: pools {tuple(shape)} and {tuple(v.shape)} are not [pages, "
+                          f"{view.page}, {n_kv_heads}, head size]")
+    if not (k.is_contiguous() and v.is_contiguous() and table.is_contiguous() and
+            ks.is_contiguous() and vs.is_contiguous()):
+        raise KernelError(f"{what}: pools, scales and page table must be contiguous")
+    if ks.dtype != torch.float32 or vs.dtype != torch.float32 or \
+            not (ks.shape == vs.shape == (pages, n_kv_heads)):
+        raise KernelError(f"{what}: scales must be float32 [{pages}, {n_kv_heads}]")
     _i32(table, "page_table")
-    return table.shape[0], table.shape[1], k.shape[0]
+    n_slots, max_pages = table.shape
+    return n_slots, max_pages, pages
 
 
 def cache_store_e4m3(k: torch.Tensor, v: torch.Tensor, view, ctx, n_kv_heads: int, head_dim: int,
@@ -2062,29 +2086,27 @@ def cache_store_e4m3(k: torch.Tensor, v: torch.Tensor, view, ctx, n_kv_heads: in
     around (a window's ring), it must leave a page more than the window takes.  A slot may
     appear once; entries with a negative slot store nothing."""
     hdv = value_dim or head_dim
-    _on_current_device(k, v, view.k_pool, view.v_pool, view.k_scale, view.v_scale, view.page_table,
-                       ctx.cu_seqlens, ctx.slots, ctx.lens)
-    T = k.shape[0]
-    _require(k.dim() == 2 and v.dim() == 2 and k.shape[1] == n_kv_heads * head_dim and
-             v.shape == (T, n_kv_heads * hdv),
-             f"cache_store_e4m3: keys {tuple(k.shape)} and values {tuple(v.shape)} do not fit "
-             f"{n_kv_heads} heads of {head_dim} and {hdv}")
-    _require(k.dtype == v.dtype, f"cache_store_e4m3: keys {k.dtype} and values {v.dtype} differ")
-    _require(k.stride(1) == 1 and v.stride(1) == 1, "cache_store_e4m3: elements of a row must be adjacent")
-    n_slots, max_pages, n_pages = _e4m3_view(view, n_kv_heads, head_dim, hdv, "cache_store_e4m3")
     cu, slots, lens = ctx.cu_seqlens, ctx.slots, ctx.lens
+    kp, vp, ks, vs, table = view.k_pool, view.v_pool, view.k_scale, view.v_scale, view.page_table
+    _on_current_device(k, v, kp, vp, ks, vs, table, cu, slots, lens)
+    T, B = k.shape[0], slots.numel()
+    if k.shape != (T, n_kv_heads * head_dim) or v.shape != (T, n_kv_heads * hdv):
+        raise KernelError(f"cache_store_e4m3: keys {tuple(k.shape)} and values {tuple(v.shape)} do "
+                          f"not fit {n_kv_heads} heads of {head_dim} and {hdv}")
+    _require(k.dtype == v.dtype, f"cache_store_e4m3: keys {k.dtype} and values {v.dtype} differ")
+    (ldk, one), (ldv, one_v) = k.stride(), v.stride()
+    _require(one == 1 and one_v == 1, "cache_store_e4m3: elements of a row must be adjacent")
+    n_slots, max_pages, n_pages = _e4m3_view(view, n_kv_heads, head_dim, hdv, "cache_store_e4m3")
     _i32(cu, "cu_seqlens"); _i32(slots, "slots"); _i32(lens, "lens")
-    B = slots.numel()
     _require(cu.numel() == B + 1 and lens.numel() == B and cu.is_contiguous() and
              slots.is_contiguous() and lens.is_contiguous(),
              "cache_store_e4m3: cu_seqlens [B + 1], slots [B] and lens [B] do not fit")
     with _span("cache_store", T * n_kv_heads * (head_dim + hdv) * (k.element_size() + 1)):
         _check(library().agv_cache_store_e4m3(
-            _ptr(k), ctypes.c_longlong(k.stride(0)), _ptr(v), ctypes.c_longlong(v.stride(0)),
-            dtype_code(k.dtype), _ptr(cu), _ptr(slots), _ptr(lens), B, T, int(ctx.max_new),
-            n_kv_heads, head_dim, hdv, _ptr(view.k_pool), _ptr(view.v_pool), _ptr(view.k_scale),
-            _ptr(view.v_scale), _ptr(view.page_table), n_slots, max_pages, view.page, view.cap,
-            n_pages, _stream()))
+            k.data_ptr(), ldk, v.data_ptr(), ldv, dtype_code(k.dtype), cu.data_ptr(),
+            slots.data_ptr(), lens.data_ptr(), B, T, int(ctx.max_new), n_kv_heads, head_dim, hdv,
+            kp.data_ptr(), vp.data_ptr(), ks.data_ptr(), vs.data_ptr(), table.data_ptr(), n_slots,
+            max_pages, view.page, view.cap, n_pages, _stream_handle()))
 
 
 def attention_decode_e4m3(q: torch.Tensor, out: torch.Tensor, view, ctx, n_heads: int,
@@ -2104,38 +2126,46 @@ def attention_decode_e4m3(q: torch.Tensor, out: torch.Tensor, view, ctx, n_heads
     _require(e4m3_head_supported(head_dim, hdv),
              f"attention_decode_e4m3: head sizes {head_dim} and {hdv} must be multiples of 16 up to "
              f"{E4M3_MAX_HEAD}")
-    _on_current_device(q, out, view.k_pool, view.v_pool, view.k_scale, view.v_scale,
-                       view.page_table, slots, positions, sinks, dist_bias)
+    kp, vp, ks, vs, table = view.k_pool, view.v_pool, view.k_scale, view.v_scale, view.page_table
+    _on_current_device(q, out, kp, vp, ks, vs, table, slots, positions, sinks, dist_bias)
     B = q.shape[0]
-    _require(q.dim() == 2 and q.shape[1] == n_heads * head_dim and q.stride(1) == 1,
-             f"attention_decode_e4m3: queries {tuple(q.shape)} are not [B, {n_heads} * {head_dim}]")
-    _require(out.dtype == q.dtype and out.is_contiguous() and out.shape == (B, n_heads * hdv),
-             f"attention_decode_e4m3: the output must be contiguous [{B}, {n_heads * hdv}] of {q.dtype}")
+    if q.shape != (B, n_heads * head_dim) or q.stride(1) != 1:
+        raise KernelError(f"attention_decode_e4m3: queries {tuple(q.shape)} are not [B, {n_heads} * "
+                          f"{head_dim}]")
+    if out.dtype != q.dtype or out.shape != (B, n_heads * hdv) or not out.is_contiguous():
+        raise KernelError(f"attention_decode_e4m3: the output must be contiguous [{B}, "
+                          f"{n_heads * hdv}] of {q.dtype}")
     n_slots, max_pages, n_pages = _e4m3_view(view, n_kv_heads, head_dim, hdv, "attention_decode_e4m3")
-    _i32(slots, "slots"); _i32(positions, "positions"); _f32(sinks, "sinks"); _f32(dist_bias, "dist_bias")
+    _i32(slots, "slots"); _i32(positions, "positions")
     _require(slots.numel() == B and positions.numel() == B and slots.is_contiguous() and
              positions.is_contiguous(), "attention_decode_e4m3: one slot and position per query")
-    _require(sinks is None or (sinks.numel() == n_heads and sinks.is_contiguous()),
-             "attention_decode_e4m3: one sink per query head")
-    _require(dist_bias is None or (dist_bias.dim() == 2 and dist_bias.shape[0] == n_heads and
-                                   dist_bias.is_contiguous()),
-             "attention_decode_e4m3: the bias by distance is [heads, distances]")
+    if sinks is not None:
+        _f32(sinks, "sinks")
+        _require(sinks.numel() == n_heads and sinks.is_contiguous(),
+                 "attention_decode_e4m3: one sink per query head")
+    n_dist = 0
+    if dist_bias is not None:
+        _f32(dist_bias, "dist_bias")
+        _require(dist_bias.dim() == 2 and dist_bias.shape[0] == n_heads and
+                 dist_bias.is_contiguous(),
+                 "attention_decode_e4m3: the bias by distance is [heads, distances]")
+        n_dist = dist_bias.shape[1]
     max_keys = max(1, min(abs(window) + keep_first, ctx.max_len) if window else ctx.max_len)
     lib = library()
     floats = lib.agv_attention_decode_e4m3_scratch(B, n_heads, n_kv_heads, head_dim, hdv, max_keys)
     if floats < 0:
         _check(floats)
     partial = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-    with _span(op, *_attention_cost(ctx, q, None, None, out, n_heads, head_dim, window, n_kv_heads,
-                                    1)):
+    cost = _attention_cost(ctx, q, None, None, out, n_heads, head_dim, window, n_kv_heads, 1)
+    with _span(op, *cost):
         _check(lib.agv_attention_decode_e4m3(
-            _ptr(q), ctypes.c_longlong(q.stride(0)), _ptr(out), dtype_code(q.dtype),
-            _ptr(view.k_pool), _ptr(view.v_pool), _ptr(view.k_scale), _ptr(view.v_scale),
-            _ptr(view.page_table), n_slots, max_pages, view.page, view.cap, n_pages, _ptr(slots),
-            _ptr(positions), B, n_heads, n_kv_heads, head_dim, hdv, ctypes.c_float(scale), window,
-            int(keep_first), _ptr(sinks), _ptr(dist_bias),
-            dist_bias.shape[1] if dist_bias is not None else 0, ctypes.c_float(softcap), max_keys,
-            _ptr(partial), ctypes.c_longlong(floats), _stream()))
+            q.data_ptr(), q.stride(0), out.data_ptr(), dtype_code(q.dtype), kp.data_ptr(),
+            vp.data_ptr(), ks.data_ptr(), vs.data_ptr(), table.data_ptr(), n_slots, max_pages,
+            view.page, view.cap, n_pages, slots.data_ptr(), positions.data_ptr(), B, n_heads,
+            n_kv_heads, head_dim, hdv, scale, window, keep_first,
+            sinks.data_ptr() if sinks is not None else None,
+            dist_bias.data_ptr() if dist_bias is not None else None, n_dist, softcap, max_keys,
+            partial.data_ptr() if partial is not None else None, floats, _stream_handle()))
 
 
 # ------------------------------------------------------------- log-probabilities
@@ -2145,15 +2175,38 @@ LOGPROBS_MAX_TOP = 32
 class TokenLogprobs:
     """What ``token_logprobs`` finds for R rows: ``logprob`` and ``entropy`` [R] (32-bit, nats),
     ``rank`` [R] (int32; 1 = the greatest logit), ``top_ids`` [R, top] (int32) and
-    ``top_logprobs`` [R, top] (32-bit), greatest first, equal ones by index."""
-    __slots__ = ("logprob", "entropy", "rank", "top_ids", "top_logprobs", "packed")
+    ``top_logprobs`` [R, top] (32-bit), greatest first, equal ones by index.  They are views of
+    ``packed``, 32 bits a value in this order, which one copy brings to the host (``unpack``)."""
+    __slots__ = ("packed", "rows", "top")
 
-    # ``packed``: all of it, 32 bits a value, in this order, so that one copy brings it to the host
+    def __init__(self, packed: torch.Tensor, rows: int, top: int):
+        self.packed, self.rows, self.top = packed, rows, top
+
+    @property
+    def logprob(self) -> torch.Tensor:
+        return self.packed[:self.rows]
+
+    @property
+    def entropy(self) -> torch.Tensor:
+        return self.packed[self.rows:2 * self.rows]
+
+    @property
+    def rank(self) -> torch.Tensor:
+        return self.packed[2 * self.rows:3 * self.rows].view(torch.int32)
+
+    @property
+    def top_ids(self) -> torch.Tensor:
+        n = self.rows * self.top
+        return self.packed[3 * self.rows:3 * self.rows + n].view(torch.int32).view(self.rows, self.top)
+
+    @property
+    def top_logprobs(self) -> torch.Tensor:
+        return self.packed[(3 + self.top) * self.rows:].view(self.rows, self.top)
+
     @staticmethod
     def unpack(packed, rows: int, top: int):
         """(logprob, entropy, rank, top ids, top logprobs) of a host copy of ``packed`` (numpy)."""
-        import numpy as np
-        i = packed.view(np.int32)
+        i = packed.view("int32")
         ids, lps = i[3 * rows:(3 + top) * rows], packed[(3 + top) * rows:(3 + 2 * top) * rows]
         return (packed[:rows], packed[rows:2 * rows], i[2 * rows:3 * rows], ids.reshape(rows, top),
                 lps.reshape(rows, top))
@@ -2170,19 +2223,12 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     R, V = logits.shape
     _i32(tokens, "tokens")
     _require(tokens.numel() == R and tokens.is_contiguous(), f"token_logprobs: one token for each of {R} rows")
-    _require(0 <= top <= min(V, LOGPROBS_MAX_TOP),
+    _require(0 <= top <= V and top <= LOGPROBS_MAX_TOP,
              f"token_logprobs: top {top} must lie in 0..{min(V, LOGPROBS_MAX_TOP)}")
-    r = TokenLogprobs()
-    # one allocation: three columns of R, two of R * top
-    floats = torch.empty((3 + 2 * top) * R, dtype=torch.float32, device=logits.device)
-    ints = floats.view(torch.int32)
-    r.logprob, r.entropy, r.rank = floats[:R], floats[R:2 * R], ints[2 * R:3 * R]
-    r.top_ids = ints[3 * R:(3 + top) * R].view(R, top)
-    r.top_logprobs = floats[(3 + top) * R:].view(R, top)
-    r.packed = floats
-    with _span("token_logprobs", _nbytes(logits, floats)):
+    packed = torch.empty((3 + 2 * top) * R, dtype=torch.float32, device=logits.device)
+    at, n = packed.data_ptr(), 4 * R
+    with _span("token_logprobs", _nbytes(logits, packed) if _perf is not None else 0):
         _check(library().agv_token_logprobs(
-            _ptr(logits), ctypes.c_longlong(logits.stride(0)), dtype_code(logits.dtype), R, V,
-            _ptr(tokens), top, _ptr(r.logprob), _ptr(r.entropy), _ptr(r.rank), _ptr(r.top_ids),
-            _ptr(r.top_logprobs), _stream()))
-    return r
+            logits.data_ptr(), logits.stride(0), dtype_code(logits.dtype), R, V, tokens.data_ptr(),
+            top, at, at + n, at + 2 * n, at + 3 * n, at + (3 + top) * n, _stream_handle()))
+    return TokenLogprobs(packed, R, top)
