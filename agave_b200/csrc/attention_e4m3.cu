@@ -51,13 +51,23 @@ struct AttendE4 {
 };
 
 // Head sizes are padded with zeros to DIM = 64, 128 or 256.
+#ifdef AE_STAGES_CTAS
+constexpr int ae_sc(int i) { const int v[6] = {S64, C64, S128, C128, S256, C256}; return v[i]; }
+#endif
 template <int DIM>
 struct Tile {
+#ifndef AE_STAGES_CTAS
     static constexpr int STAGES = DIM == 64 ? 4 : 3;
     static constexpr int CTAS = DIM == 256 ? 2 : DIM == 128 ? 3 : 5;     // resident on an SM
-    // Row strides by which a warp's 16-byte reads meet every bank once: two key rows of 64 bytes,
-    // four value rows of 32.
-    static constexpr int KS = DIM == 64 ? 64 : DIM + 64, VS = DIM + 16;
+#else
+
+    static constexpr int STAGES = ae_sc(DIM == 64 ? 0 : DIM == 128 ? 2 : 4);
+    static constexpr int CTAS = ae_sc(DIM == 64 ? 1 : DIM == 128 ? 3 : 5);
+#endif
+    // A warp's 16-byte reads meet every bank once: of two key rows 64 bytes each, which lie in
+    // different halves of 128 bytes (odd rows of 128 bytes or more have them exchanged), of four
+    // value rows 32 bytes each, by the stride.
+    static constexpr int KS = DIM, VS = DIM + 16;
     static constexpr int STAGE = 16 * (KS + VS);
     static constexpr int RED = DIM + 4;                                   // floats
     static constexpr int SMEM = AE_WARPS * STAGES * STAGE;
@@ -331,7 +341,8 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
             };
             constexpr int LPR = DIM / 16, RPI = 32 / LPR;        // lanes a row, rows an instruction
             const int crow = lane / LPR, ccol = lane % LPR * 16;
-            const unsigned copy_at = mine_at + crow * S::KS + ccol, copy_vat = mine_at + 16 * S::KS + crow * S::VS + ccol;
+            const int flip = DIM > 64 ? (crow & 1) * 64 : 0;
+            const unsigned copy_at = mine_at + crow * S::KS + (ccol ^ flip), copy_vat = mine_at + 16 * S::KS + crow * S::VS + ccol;
             const int k_bytes = ccol < a.hd ? 16 : 0, v_bytes = ccol < a.hdv ? 16 : 0;
             const unsigned char* k_from = a.k_pool + (size_t)crow * krow + (size_t)g * a.hd + (k_bytes ? ccol : 0);
             const unsigned char* v_from = a.v_pool + (size_t)crow * vrow + (size_t)g * a.hdv + (v_bytes ? ccol : 0);
@@ -450,15 +461,17 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
                 __syncwarp();
                 const int j0 = now.j;
                 if (j0 <= s.p && meta[warp][stage][2] != 0.f) {
-                    const unsigned char* K = mine + stage * S::STAGE;
-                    const unsigned char* V = K + 16 * S::KS;
+                    const unsigned char* V = mine + stage * S::STAGE + 16 * S::KS;
+                    const unsigned char* K = mine + stage * S::STAGE + r * S::KS + c * 16;
+                    const int half = DIM > 64 ? (r & 1) * 64 : 0;
                     const float ks = meta[warp][stage][0], vs = meta[warp][stage][1];
                     float x[2][4] = {};
                     float y[2][4] = {};
 #pragma unroll
                     for (int q = 0; q < NQ; ++q) {
-                        const uint4 ka = *reinterpret_cast<const uint4*>(K + r * S::KS + q * 64 + c * 16);
-                        const uint4 kb = *reinterpret_cast<const uint4*>(K + (r + 8) * S::KS + q * 64 + c * 16);
+                        const unsigned char* at = K + q * 64 + (q & 1 ? -half : half);
+                        const uint4 ka = *reinterpret_cast<const uint4*>(at);
+                        const uint4 kb = *reinterpret_cast<const uint4*>(at + 8 * S::KS);
                         const unsigned wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
                         for (int f = 0; f < 4; ++f) {

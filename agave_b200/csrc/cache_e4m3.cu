@@ -4,6 +4,11 @@
 // magnitude of the new rows there gives the scale, the rows are rounded to codes.  Where the
 // page already holds earlier tokens of the sequence the scale never shrinks, and if it
 // grows their codes are rounded to the greater one.
+//
+// What bounds it is reading the rows once and writing a byte for each value.  Prompts: a page's
+// rows (64 of 256 values: 32 KB of bfloat16) stay in registers between the maximum and the
+// rounding, read 16 bytes at a time.  Single tokens, and rows that do not start on 16 bytes, go two values
+// at a time and are read twice (the second time from L1); there it is the launch that counts.
 #include "e4m3.cuh"
 
 namespace {
@@ -20,8 +25,31 @@ struct StoreE4 {
     int T, n_slots, max_pages, n_pages, page, cap, nkv;
 };
 
+// Scale of a page and head from the new rows' magnitude and, where the page goes on (r0 rows of it
+// are held), the scale it has; the held codes move to it if it grows.  All threads of the CTA.
+__device__ __forceinline__ float settle_scale(float amax, float* sc, int r0, unsigned char* codes, size_t row, int dim) {
+    float s = e4m3_scale(amax);
+    if (r0 > 0) {
+        const float old = *sc;
+        s = fmaxf(s, old);
+        if (s != old) {
+            const float f = old * e4m3_inverse(s);
+            const int quads = dim / 4;
+            for (int i = threadIdx.x; i < r0 * quads; i += blockDim.x) {
+                unsigned* e = (unsigned*)(codes + (size_t)(i / quads) * row) + i % quads;
+                const unsigned w = *e;
+                const float2 lo = e4m3_to_float2(w), hi = e4m3_to_float2(w >> 16);
+                *e = e4m3_pair(lo.x * f, lo.y * f) | e4m3_pair(hi.x * f, hi.y * f) << 16;
+            }
+        }
+        __syncthreads();                           // everyone has read the old scale
+    }
+    if (threadIdx.x == 0) *sc = s;
+    return s;
+}
+
 template <typename T>
-__global__ void __launch_bounds__(CE_THREADS) store_e4m3_kernel(StoreE4 a) {
+__global__ void __launch_bounds__(CE_THREADS) store_e4m3_kernel(const StoreE4 a) {
     pdl_wait();
     pdl_launch_next();
     __shared__ float scratch[32];
@@ -46,22 +74,8 @@ __global__ void __launch_bounds__(CE_THREADS) store_e4m3_kernel(StoreE4 a) {
             amax = fmaxf(amax, fmaxf(e4m3_magnitude(to_f32(e[0])), e4m3_magnitude(to_f32(e[1]))));
         }
         amax = block_max(amax, scratch);
-        float s = e4m3_scale(amax);
         const int r0 = p0 - j * a.page;
-        if (r0 > 0) {
-            const float old = *sc;
-            s = fmaxf(s, old);
-            if (s != old) {
-                const float f = old * e4m3_inverse(s);
-                for (int i = tid; i < r0 * half; i += CE_THREADS) {
-                    unsigned short* e = (unsigned short*)(dst + (size_t)(i / half) * a.nkv * dim) + i % half;
-                    const float2 v = e4m3_to_float2(*e);
-                    *e = (unsigned short)e4m3_pair(v.x * f, v.y * f);
-                }
-            }
-        }
-        __syncthreads();                           // everyone has read the old scale
-        if (tid == 0) *sc = s;
+        const float s = settle_scale(amax, sc, r0, dst, (size_t)a.nkv * dim, dim);
         const float inv = e4m3_inverse(s);
         for (int i = tid; i < pairs; i += CE_THREADS) {
             const T* e = src + (long long)(i / half) * a.ld[which] + i % half * 2;
@@ -69,6 +83,125 @@ __global__ void __launch_bounds__(CE_THREADS) store_e4m3_kernel(StoreE4 a) {
                 (unsigned short)e4m3_pair(to_f32(e[0]) * inv, to_f32(e[1]) * inv);
         }
     }
+}
+
+// The same for rows of 16-byte pieces, pages of at most 64 positions and dimensions of at most 256:
+// the page's rows in registers.  ``PIECES``: 16-byte pieces a thread holds.
+constexpr int CP_THREADS = 256;
+
+// The greatest magnitude of 16 bytes of values (infinity if one is infinite; NaN does not count).
+__device__ __forceinline__ float piece_max(const uint4& u, float) {
+    return fmaxf(fmaxf(fabsf(__uint_as_float(u.x)), fabsf(__uint_as_float(u.y))),
+                 fmaxf(fabsf(__uint_as_float(u.z)), fabsf(__uint_as_float(u.w))));
+}
+__device__ __forceinline__ __nv_bfloat162 pair_of(unsigned w) {
+    return *reinterpret_cast<const __nv_bfloat162*>(&w);
+}
+__device__ __forceinline__ float piece_max(const uint4& u, __nv_bfloat16) {
+    const __nv_bfloat162 m = __hmax2(__hmax2(__habs2(pair_of(u.x)), __habs2(pair_of(u.y))),
+                                     __hmax2(__habs2(pair_of(u.z)), __habs2(pair_of(u.w))));
+    return fmaxf(__low2float(m), __high2float(m));
+}
+template <typename T>
+__device__ __forceinline__ void piece_values(const uint4& u, float (&x)[16 / sizeof(T)]) {
+    const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            x[i] = __uint_as_float(w[i]);
+        } else {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+}
+// (an infinity saturates here: for values that are known to have none)
+__device__ __forceinline__ unsigned e4m3_pair_finite(float a, float b) {
+    unsigned short r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
+    return r;
+}
+
+template <typename T, int PIECES>
+__global__ void __launch_bounds__(CP_THREADS) store_pages_e4m3_kernel(const StoreE4 a) {
+    constexpr int N = 16 / sizeof(T);
+    pdl_wait();
+    pdl_launch_next();
+    __shared__ float scratch[32];
+    const int b = blockIdx.z, which = blockIdx.y & 1, g = blockIdx.y >> 1, tid = threadIdx.x;
+    const int slot = a.slots[b], c0 = a.cu[b], n = a.cu[b + 1] - c0, len = a.lens[b];
+    if (slot < 0 || slot >= a.n_slots || n <= 0 || c0 < 0 || c0 > a.T - n || len < n) return;
+    const int start = len - n, last = (len - 1) / a.page;
+    const int first = max(start / a.page, last - a.cap / a.page + 1);
+    const int dim = a.dim[which], per_row = dim / N;
+    // this thread's pieces: (row, column) and the step from one to the next
+    const int row0 = tid / per_row, col0 = tid % per_row, row_step = CP_THREADS / per_row, col_step = CP_THREADS % per_row;
+    const long long ld = a.ld[which];
+    for (int j = first + blockIdx.x; j <= last; j += gridDim.x) {
+        const int p0 = max(start, j * a.page), rows = min(len, (j + 1) * a.page) - p0;
+        const int page = a.table[(size_t)slot * a.max_pages + j % (a.cap / a.page)];
+        if (page < 0 || page >= a.n_pages) continue;
+        const T* src = (const T*)a.x[which] + (long long)(c0 + p0 - start) * ld + (size_t)g * dim;
+        unsigned char* dst = a.pool[which] + ((size_t)page * a.page * a.nkv + g) * dim;
+        const size_t drow = (size_t)a.nkv * dim;
+        uint4 u[PIECES];
+        float amax = 0.f;
+        int r = row0, c = col0;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            u[i] = r < rows ? __ldg(reinterpret_cast<const uint4*>(src + r * ld) + c) : make_uint4(0, 0, 0, 0);
+            r += row_step;
+            c += col_step;
+            if (c >= per_row) { c -= per_row; ++r; }
+        }
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) amax = fmaxf(amax, piece_max(u[i], T{}));
+        amax = block_max(amax, scratch);
+        const bool infinite = amax == INFINITY;
+        if (infinite) {                            // the greatest of the finite ones
+            amax = 0.f;
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                float x[N];
+                piece_values<T>(u[i], x);
+#pragma unroll
+                for (int e = 0; e < N; ++e) amax = fmaxf(amax, e4m3_magnitude(x[e]));
+            }
+            amax = block_max(amax, scratch);
+        }
+        const int r0 = p0 - j * a.page;
+        const float inv = e4m3_inverse(settle_scale(amax, a.scale[which] + (size_t)page * a.nkv + g, r0, dst, drow, dim));
+        dst += r0 * drow;
+        r = row0;
+        c = col0;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            if (r < rows) {
+                float x[N];
+                piece_values<T>(u[i], x);
+                unsigned w[N / 4];
+#pragma unroll
+                for (int e = 0; e < N / 4; ++e) {
+                    const float x0 = x[4 * e] * inv, x1 = x[4 * e + 1] * inv, x2 = x[4 * e + 2] * inv, x3 = x[4 * e + 3] * inv;
+                    w[e] = infinite ? e4m3_pair(x0, x1) | e4m3_pair(x2, x3) << 16
+                                    : e4m3_pair_finite(x0, x1) | e4m3_pair_finite(x2, x3) << 16;
+                }
+                unsigned* to = reinterpret_cast<unsigned*>(dst + r * drow) + c * (N / 4);
+                if constexpr (N == 8) *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+                else *to = w[0];
+            }
+            r += row_step;
+            c += col_step;
+            if (c >= per_row) { c -= per_row; ++r; }
+        }
+    }
+}
+template <typename T>
+void launch_pages(const StoreE4& a, dim3 grid, int dim, cudaStream_t stream) {
+    constexpr int ALL = 64 * 256 * sizeof(T) / 16 / CP_THREADS;      // pieces of the greatest page: 8 or 16
+    if (dim > 128) agv_launch(store_pages_e4m3_kernel<T, ALL>, grid, CP_THREADS, 0, stream, a);
+    else if (dim > 64) agv_launch(store_pages_e4m3_kernel<T, ALL / 2>, grid, CP_THREADS, 0, stream, a);
+    else agv_launch(store_pages_e4m3_kernel<T, ALL / 4>, grid, CP_THREADS, 0, stream, a);
 }
 
 }  // namespace
@@ -98,6 +231,15 @@ AGV_API int agv_cache_store_e4m3(const void* k, long long ldk, const void* v, lo
     int blocks = most == 1 ? 1 : (most + page - 2) / page + 1;
     if (blocks > cap / page) blocks = cap / page;
     const dim3 grid(blocks, 2 * nkv, B);
+    const size_t esz = dtype == AGV_F32 ? 4 : 2;
+    const int most_dim = hd > hdv ? hd : hdv;
+    if (most > 1 && page <= 64 && most_dim <= 256 && agv_aligned(k, 16) && agv_aligned(v, 16) && ldk * esz % 16 == 0 &&
+        ldv * esz % 16 == 0) {
+        if (dtype == AGV_F32) launch_pages<float>(a, grid, most_dim, stream);
+        else launch_pages<__nv_bfloat16>(a, grid, most_dim, stream);
+        AGV_LAUNCH_OK("store_pages_e4m3_kernel");
+        return 0;
+    }
     if (dtype == AGV_F32) agv_launch(store_e4m3_kernel<float>, grid, CE_THREADS, 0, stream, a);
     else agv_launch(store_e4m3_kernel<__nv_bfloat16>, grid, CE_THREADS, 0, stream, a);
     AGV_LAUNCH_OK("store_e4m3_kernel");

@@ -7,14 +7,16 @@
 // log2 e of the exponential: logits may be the type's lowest value.)
 //
 // What bounds it is reading the logits once.  A row is the work of a cluster of 1 to 16 CTAs; a
-// thread takes every LP_THREADS-th 16 bytes of its CTA's slice, four of them under way, and keeps a
-// running maximum, the two sums and the count of logits ahead of the token's.
+// thread takes every LP_THREADS-th 16 bytes of its CTA's slice, four of them while the next four are
+// under way, and keeps a running maximum, the two sums and the count of logits ahead of the
+// token's; the arithmetic goes two values an instruction where there is one for two.
 //
-// The greatest: a logit and its index are one 64-bit key.  Every thread knows the greatest key
-// it has seen (the running maximum tells it when to look), so the top-th greatest of the threads' keys
-// is a bound that at least ``top`` keys of the slice reach, and beside those threads' own keys hardly
-// any other does.  The slices of the few threads that reach it are read once more (from
-// L2) and ranked; the cluster's first CTA merges the slices' lists.
+// The greatest: a logit and its index are one 64-bit key.  Every thread knows its maximum and in
+// which four pieces it stood, that is, a key that its greatest logit reaches.  Of the greatest
+// such keys of LP_GROUPS groups of threads the top-th is a bound that at least ``top`` keys of the
+// slice reach, and few others do (of 64 groups and top 20 some 4 more).  The pieces of the threads
+// that may reach it are read once more (from L2) and what does is ranked; the cluster's first CTA
+// merges the slices' lists.
 #include "common.cuh"
 
 namespace {
@@ -23,6 +25,8 @@ constexpr int LP_THREADS = 512;
 constexpr int LP_WARPS = LP_THREADS / 32;
 constexpr int LP_MAX_TOP = 32;
 constexpr int LP_MAX_CLUSTER = 16;
+constexpr int LP_GROUPS = 64;
+constexpr int LP_GROUP_LANES = LP_THREADS / LP_GROUPS;
 constexpr int LP_LIST = 2048;             // keys at or above the bound that a CTA can list
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -47,6 +51,11 @@ __device__ __forceinline__ float lp_ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
 }
 __device__ __forceinline__ float max_nan(float a, float b) {        // NaN if either is
     float y;
@@ -122,58 +131,46 @@ __device__ __forceinline__ void put(unsigned at, u64 v) {
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory");
 }
 
-// 16 bytes of logits
+// 16 bytes of logits as pairs of 32-bit values, and the greatest of them.
 template <typename T> struct Piece;
 template <> struct Piece<float> {
     static constexpr int N = 4;
-    static __device__ __forceinline__ void load(const float* p, float* x) {
-        const float4 v = __ldg(reinterpret_cast<const float4*>(p));
-        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    static __device__ __forceinline__ void values(const uint4& u, float* x) {
+        x[0] = __uint_as_float(u.x); x[1] = __uint_as_float(u.y);
+        x[2] = __uint_as_float(u.z); x[3] = __uint_as_float(u.w);
+    }
+    static __device__ __forceinline__ float greatest(const uint4& u) {
+        return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
     }
 };
 template <> struct Piece<__nv_bfloat16> {
     static constexpr int N = 8;
-    static __device__ __forceinline__ void load(const __nv_bfloat16* p, float* x) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-        const unsigned w[4] = {v.x, v.y, v.z, v.w};
+    static __device__ __forceinline__ void values(const uint4& u, float* x) {
+        const unsigned w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             x[2 * i] = __uint_as_float(w[i] << 16);
             x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
         }
     }
-};
-
-// The 32 keys of a warp's lanes, greatest first (a bitonic sort).
-__device__ __forceinline__ u64 sorted(u64 k, int lane) {
-#pragma unroll
-    for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-        for (int o = size >> 1; o > 0; o >>= 1) {
-            const u64 p = __shfl_xor_sync(0xffffffffu, k, o);
-            const bool up = (lane & o) == 0, down = (lane & size) == 0 || size == 32;
-            k = (up == down) == (p > k) ? p : k;
-        }
-    return k;
-}
-// The same for keys that rise and then fall (or the other way round).
-__device__ __forceinline__ u64 sorted_bitonic(u64 k, int lane) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const u64 p = __shfl_xor_sync(0xffffffffu, k, o);
-        k = ((lane & o) == 0) == (p > k) ? p : k;
+    static __device__ __forceinline__ __nv_bfloat162 pair(unsigned w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); }
+    static __device__ __forceinline__ float greatest(const uint4& u) {
+        const __nv_bfloat162 m = __hmax2(__hmax2(pair(u.x), pair(u.y)), __hmax2(pair(u.z), pair(u.w)));
+        return fmaxf(__low2float(m), __high2float(m));
     }
-    return k;
-}
+};
+__device__ __forceinline__ uint4 piece_at(const void* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
 
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(LP_THREADS, 2) logprobs_kernel(const Logprobs a) {
-    constexpr int N = Piece<T>::N, BATCH = 16 / N;         // 16 logits under way, and 64 or 32 bytes
+    constexpr int N = Piece<T>::N, BATCH = 4;
     __shared__ Sums wsum[LP_WARPS];
     __shared__ int wahead[LP_WARPS];
     __shared__ Slice slices[LP_MAX_CLUSTER];               // the first CTA's count
-    __shared__ u64 merge[TOP ? LP_WARPS : 1][32];
+    __shared__ u64 group_best[TOP ? LP_GROUPS : 1];
     __shared__ u64 list[TOP ? LP_LIST : 1];
+    __shared__ u64 greatest[TOP ? LP_MAX_TOP : 1];         // of the slice, in order
+    __shared__ u64 warp_best[TOP ? LP_WARPS : 1];
     __shared__ int n_list;
     __shared__ u64 bound_key;
     const int C = a.cluster;
@@ -183,63 +180,95 @@ __global__ void __launch_bounds__(LP_THREADS, 2) logprobs_kernel(const Logprobs 
     const int row = blockIdx.x / C, rank = C > 1 ? (int)lp_cluster_rank() : 0;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const T* x = (const T*)a.logits + (long long)row * a.ld;
-    const int tok = a.tokens[row];
-    const bool has = tok >= 0 && tok < a.V;
-    const float xt = has ? to_f32(x[tok]) : INFINITY;
     // the row as 16-byte pieces behind a head that ends at a 16-byte boundary
     const int head = min(a.V, (int)((16 - (uintptr_t)x % 16) % 16 / sizeof(T)));
     const int pieces = (a.V - head) / N, per = (pieces + C - 1) / C;
     const int v0 = min(pieces, rank * per), v1 = min(pieces, v0 + per);
+    const T* body = x + head;
+
+    int v = v0 + tid;
+    uint4 next[BATCH];
+    auto fetch = [&]() {
+#pragma unroll
+        for (int q = 0; q < BATCH; ++q) next[q] = piece_at(body + (size_t)(v + q * LP_THREADS) * N);
+    };
+    bool full = v + (BATCH - 1) * LP_THREADS < v1;
+    if (full) fetch();                                     // (before the token's logit is asked for)
+    const int tok = a.tokens[row];
+    const bool has = tok >= 0 && tok < a.V;
+    const float xt = has ? to_f32(x[tok]) : INFINITY;
 
     Sums sum{-INFINITY, 0.f, 0.f};
     float m = -INFINITY;
-    u64 best = 0;
+    int m_at = -1;                                         // index where the pieces with the maximum begin
     int ahead = 0;
-    // x[0 .. n) of indices i, i + 1, ... (in pieces of N, LP_THREADS pieces apart)
-    auto take = [&](const float* v, auto n_const, int i) {
+    // the values of n pieces, LP_THREADS apart, that begin at index i
+    auto take = [&](const uint4* u, auto n_const, int i) {
         constexpr int n = decltype(n_const)::value;
-        float bm = v[0];
+        float bm = Piece<T>::greatest(u[0]);
 #pragma unroll
-        for (int e = 1; e < n; ++e) bm = fmaxf(bm, v[e]);
-        if (bm > m || (TOP && best == 0)) {
-            if (TOP) {
-#pragma unroll
-                for (int e = 0; e < n; ++e)
-                    best = greater(best, lp_key(v[e], i + e / N * (LP_THREADS * N) + e % N));
-            }
-            if (bm > m) {
-                m = bm;
-                sum.move(m);
-            }
+        for (int q = 1; q < n; ++q) bm = fmaxf(bm, Piece<T>::greatest(u[q]));
+        if (bm > m || (bm == m && m_at < 0)) m_at = i;
+        if (bm > m) {
+            m = bm;
+            sum.move(m);
         }
         const float c = sum.c == -INFINITY ? 0.f : sum.c;
+        const f32x2 minus_c = pack2(-c, -c), log2e = pack2(LOG2E, LOG2E);
+        f32x2 s = pack2(0.f, 0.f), w = pack2(0.f, 0.f);
 #pragma unroll
-        for (int e = 0; e < n; ++e) {
-            // (at e^-150 a term is 0 and its product with d is, too)
-            const float d = max_nan(v[e] - c, -150.f), p = lp_ex2(d * LOG2E);
-            sum.s += p;
-            sum.t = fmaf(p, d, sum.t);
+        for (int q = 0; q < n; ++q) {
+            float x[N];
+            Piece<T>::values(u[q], x);
+#pragma unroll
+            for (int e = 0; e < N; e += 2) {
+                // (at e^-150 a term is 0 and its product with d is, too)
+                float d0, d1, y0, y1;
+                unpack2(add2(pack2(x[e], x[e + 1]), minus_c), d0, d1);
+                const f32x2 d = pack2(max_nan(d0, -150.f), max_nan(d1, -150.f));
+                unpack2(mul2(d, log2e), y0, y1);
+                const f32x2 p = pack2(lp_ex2(y0), lp_ex2(y1));
+                s = add2(s, p);
+                w = fma2(p, d, w);
+            }
         }
+        float lo, hi;
+        unpack2(s, lo, hi);
+        sum.s += lo + hi;
+        unpack2(w, lo, hi);
+        sum.t += lo + hi;
         if (bm >= xt) {
+            const int end = i + (n - 1) * LP_THREADS * N + N;
 #pragma unroll
-            for (int e = 0; e < n; ++e) {
-                const int at = i + e / N * (LP_THREADS * N) + e % N;
-                ahead += v[e] > xt || (v[e] == xt && at < tok);
+            for (int q = 0; q < n; ++q) {
+                float x[N];
+                Piece<T>::values(u[q], x);
+                if (i > tok) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) ahead += x[e] > xt;
+                } else if (end <= tok) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) ahead += x[e] >= xt;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) ahead += x[e] > xt || (x[e] == xt && i + q * LP_THREADS * N + e < tok);
+                }
             }
         }
     };
-    const T* body = x + head;
-    int v = v0 + tid;
-    for (; v + (BATCH - 1) * LP_THREADS < v1; v += BATCH * LP_THREADS) {
-        float w[BATCH * N];
+    while (full) {
+        uint4 u[BATCH];
 #pragma unroll
-        for (int q = 0; q < BATCH; ++q) Piece<T>::load(body + (size_t)(v + q * LP_THREADS) * N, w + q * N);
-        take(w, std::integral_constant<int, BATCH * N>{}, head + v * N);
+        for (int q = 0; q < BATCH; ++q) u[q] = next[q];
+        const int i = head + v * N;
+        v += BATCH * LP_THREADS;
+        full = v + (BATCH - 1) * LP_THREADS < v1;
+        if (full) fetch();
+        take(u, std::integral_constant<int, BATCH>{}, i);
     }
     for (; v < v1; v += LP_THREADS) {
-        float w[N];
-        Piece<T>::load(body + (size_t)v * N, w);
-        take(w, std::integral_constant<int, N>{}, head + v * N);
+        const uint4 u = piece_at(body + (size_t)v * N);
+        take(&u, std::integral_constant<int, 1>{}, head + v * N);
     }
     // the head and what is left behind the last piece: a thread of the first CTA each
     const int tail = a.V - head - pieces * N;
@@ -248,7 +277,15 @@ __global__ void __launch_bounds__(LP_THREADS, 2) logprobs_kernel(const Logprobs 
     float xe = 0.f;
     if (edge >= 0) {
         xe = to_f32(x[edge]);
-        take(&xe, std::integral_constant<int, 1>{}, edge);
+        if (xe > m || (xe == m && m_at < 0)) m_at = edge;
+        if (xe > m) {
+            m = xe;
+            sum.move(m);
+        }
+        const float d = max_nan(xe - (sum.c == -INFINITY ? 0.f : sum.c), -150.f), p = lp_ex2(d * LOG2E);
+        sum.s += p;
+        sum.t = fmaf(p, d, sum.t);
+        ahead += xe > xt || (xe == xt && edge < tok);
     }
     // ---- sums and counts of the CTA
 #pragma unroll
@@ -262,14 +299,23 @@ __global__ void __launch_bounds__(LP_THREADS, 2) logprobs_kernel(const Logprobs 
         wsum[warp] = sum;
         wahead[warp] = ahead;
     }
-    if (tid == 0) n_list = 0;
-    u64 k = 0;
+    // The maximum stands at m_at or up to SPAN indices behind it: a key it reaches, and one that
+    // nothing of the thread exceeds.
+    constexpr unsigned SPAN = (BATCH - 1) * LP_THREADS * N + N - 1;
+    const u64 reached = m_at < 0 ? 0 : lp_key(m, m_at + SPAN), most = m_at < 0 ? 0 : lp_key(m, m_at);
     if (TOP) {
-        k = sorted(best, lane);
-        merge[warp][lane] = k;
+        u64 k = reached;
+#pragma unroll
+        for (int o = 1; o < LP_GROUP_LANES; o <<= 1) k = greater(k, __shfl_xor_sync(0xffffffffu, k, o));
+        if (tid % LP_GROUP_LANES == 0) group_best[tid / LP_GROUP_LANES] = k;
+        if (tid == 0) {
+            n_list = 0;
+            bound_key = 0;
+        }
+        if (tid < LP_MAX_TOP) greatest[tid] = 0;
     }
     __syncthreads();
-    if (warp == 0) {
+    if (warp == LP_WARPS - 1) {
         Sums all = wsum[lane & (LP_WARPS - 1)];
         int n = wahead[lane & (LP_WARPS - 1)];
 #pragma unroll
@@ -279,20 +325,17 @@ __global__ void __launch_bounds__(LP_THREADS, 2) logprobs_kernel(const Logprobs 
             all.join(oc, os, ot);
             n += __shfl_xor_sync(0xffffffffu, n, o);
         }
-        sum = all;                                         // lane 0's is handed on below
+        sum = all;                                         // handed on below
         ahead = n;
     }
     if (TOP) {
-        // the greatest 32 of two warps' sorted keys, four times
-#pragma unroll
-        for (int d = 1; d < LP_WARPS; d <<= 1) {
-            if ((warp & (2 * d - 1)) == 0) {
-                k = sorted_bitonic(greater(k, merge[warp + d][31 - lane]), lane);
-                merge[warp][lane] = k;
-            }
-            __syncthreads();
+        if (tid < LP_GROUPS) {
+            const u64 k = group_best[tid];
+            int before = 0;
+#pragma unroll 8
+            for (int j = 0; j < LP_GROUPS; ++j) before += group_best[j] > k;
+            if (before == a.top - 1 && k) bound_key = k;
         }
-        if (warp == 0 && lane == a.top - 1) bound_key = k;
         __syncthreads();
         const u64 bound = bound_key;
         auto note = [&](u64 key) {
@@ -301,27 +344,25 @@ __global__ void __launch_bounds__(LP_THREADS, 2) logprobs_kernel(const Logprobs 
             if (at < LP_LIST) list[at] = key;
         };
         if (edge >= 0) note(lp_key(xe, edge));
-        // the pieces of a thread that reaches the bound, a lane each
-        for (unsigned who = __ballot_sync(0xffffffffu, best >= bound); who; who &= who - 1) {
+        // the pieces of a thread that may reach the bound, a lane each
+        for (unsigned who = __ballot_sync(0xffffffffu, most >= bound); who; who &= who - 1) {
             const int first = v0 + (tid & ~31) + __ffs(who) - 1;
             for (int p = first + lane * LP_THREADS; p < v1; p += 32 * LP_THREADS) {
                 float w[N];
-                Piece<T>::load(body + (size_t)p * N, w);
+                Piece<T>::values(piece_at(body + (size_t)p * N), w);
 #pragma unroll
                 for (int e = 0; e < N; ++e) note(lp_key(w[e], head + p * N + e));
             }
         }
         __syncthreads();
         const int n = n_list;
-        u64* out = merge[0];                               // the slice's list, greatest first, 0 behind its end
-        if (tid < 32) out[tid] = 0;
-        __syncthreads();
         if (n <= LP_LIST) {
             for (int i = tid; i < n; i += LP_THREADS) {
                 const u64 key = list[i];
                 int before = 0;
+#pragma unroll 4
                 for (int j = 0; j < n; ++j) before += list[j] > key;
-                if (before < a.top) out[before] = key;
+                if (before < a.top) greatest[before] = key;
             }
         } else {
             // more than the list holds: one after the other from the logits
@@ -330,19 +371,20 @@ __global__ void __launch_bounds__(LP_THREADS, 2) logprobs_kernel(const Logprobs 
                 u64 mine = edge >= 0 && lp_key(xe, edge) < below ? lp_key(xe, edge) : 0;
                 for (int p = v0 + tid; p < v1; p += LP_THREADS) {
                     float w[N];
-                    Piece<T>::load(body + (size_t)p * N, w);
+                    Piece<T>::values(piece_at(body + (size_t)p * N), w);
 #pragma unroll
                     for (int e = 0; e < N; ++e) {
                         const u64 key = lp_key(w[e], head + p * N + e);
                         if (key < below) mine = greater(mine, key);
                     }
                 }
-                mine = sorted(mine, lane);
-                if (lane == 0) merge[1][warp] = mine;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) mine = greater(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+                if (lane == 0) warp_best[warp] = mine;
                 __syncthreads();
-                below = merge[1][0];
-                for (int w = 1; w < LP_WARPS; ++w) below = greater(below, merge[1][w]);
-                if (tid == 0) out[q] = below;
+                below = warp_best[0];
+                for (int w = 1; w < LP_WARPS; ++w) below = greater(below, warp_best[w]);
+                if (tid == 0) greatest[q] = below;
                 __syncthreads();
             }
         }
@@ -351,13 +393,13 @@ __global__ void __launch_bounds__(LP_THREADS, 2) logprobs_kernel(const Logprobs 
     // ---- to the first CTA of the cluster
     if (C > 1) lp_cluster_wait();
     Slice* at = &slices[rank];
-    if (tid == 0) {
+    if (tid == LP_THREADS - 1) {
         put(in_first_cta(&at->c), sum.c);
         put(in_first_cta(&at->s), sum.s);
         put(in_first_cta(&at->t), sum.t);
         put(in_first_cta(&at->ahead), ahead);
     }
-    if (TOP && tid < a.top) put(in_first_cta(&at->keys[tid]), merge[0][tid]);
+    if (TOP && tid < a.top) put(in_first_cta(&at->keys[tid]), greatest[tid]);
     if (C > 1) {
         lp_cluster_arrive();
         lp_cluster_wait();
