@@ -53,14 +53,15 @@ __global__ void __launch_bounds__(CE_THREADS) store_e4m3_kernel(const StoreE4 a)
     pdl_wait();
     pdl_launch_next();
     __shared__ float scratch[32];
-    const int b = blockIdx.z, which = blockIdx.y & 1, g = blockIdx.y >> 1, tid = threadIdx.x;
+    // (the heads of a page beside each other on the grid: together their rows are whole)
+    const int b = blockIdx.z, which = blockIdx.x / a.nkv, g = blockIdx.x % a.nkv, tid = threadIdx.x;
     const int slot = a.slots[b], c0 = a.cu[b], n = a.cu[b + 1] - c0, len = a.lens[b];
     if (slot < 0 || slot >= a.n_slots || n <= 0 || c0 < 0 || c0 > a.T - n || len < n) return;
     const int start = len - n, last = (len - 1) / a.page;
     const int first = max(start / a.page, last - a.cap / a.page + 1);
     const int dim = a.dim[which];
     const T* x = (const T*)a.x[which] + (size_t)g * dim;
-    for (int j = first + blockIdx.x; j <= last; j += gridDim.x) {
+    for (int j = first + blockIdx.y; j <= last; j += gridDim.y) {
         const int p0 = max(start, j * a.page), p1 = min(len, (j + 1) * a.page);
         const int page = a.table[(size_t)slot * a.max_pages + j % (a.cap / a.page)];
         if (page < 0 || page >= a.n_pages) continue;
@@ -86,8 +87,7 @@ __global__ void __launch_bounds__(CE_THREADS) store_e4m3_kernel(const StoreE4 a)
 }
 
 // The same for rows of 16-byte pieces, pages of at most 64 positions and dimensions of at most 256:
-// the page's rows in registers.  ``PIECES``: 16-byte pieces a thread holds.
-constexpr int CP_THREADS = 256;
+// the page's rows in registers, 1 to 8 pieces a thread.
 
 // The greatest magnitude of 16 bytes of values (infinity if one is infinite; NaN does not count).
 __device__ __forceinline__ float piece_max(const uint4& u, float) {
@@ -122,38 +122,45 @@ __device__ __forceinline__ unsigned e4m3_pair_finite(float a, float b) {
     return r;
 }
 
-template <typename T, int PIECES>
-__global__ void __launch_bounds__(CP_THREADS) store_pages_e4m3_kernel(const StoreE4 a) {
+template <typename T, int PIECES, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) store_pages_e4m3_kernel(const StoreE4 a) {
     constexpr int N = 16 / sizeof(T);
     pdl_wait();
     pdl_launch_next();
     __shared__ float scratch[32];
-    const int b = blockIdx.z, which = blockIdx.y & 1, g = blockIdx.y >> 1, tid = threadIdx.x;
+    // (the heads of a page beside each other on the grid: together their rows are whole)
+    const int b = blockIdx.z, which = blockIdx.x / a.nkv, g = blockIdx.x % a.nkv, tid = threadIdx.x;
     const int slot = a.slots[b], c0 = a.cu[b], n = a.cu[b + 1] - c0, len = a.lens[b];
     if (slot < 0 || slot >= a.n_slots || n <= 0 || c0 < 0 || c0 > a.T - n || len < n) return;
     const int start = len - n, last = (len - 1) / a.page;
     const int first = max(start / a.page, last - a.cap / a.page + 1);
     const int dim = a.dim[which], per_row = dim / N;
-    // this thread's pieces: (row, column) and the step from one to the next
-    const int row0 = tid / per_row, col0 = tid % per_row, row_step = CP_THREADS / per_row, col_step = CP_THREADS % per_row;
-    const long long ld = a.ld[which];
-    for (int j = first + blockIdx.x; j <= last; j += gridDim.x) {
+    // this thread's pieces, THREADS apart in the order of rows: the first one's row and column, and
+    // the steps to the next
+    const int row0 = tid / per_row, col0 = tid % per_row, row_step = THREADS / per_row, col_step = THREADS % per_row;
+    const long long ld = a.ld[which], drow = (long long)a.nkv * dim;
+    const long long x_step = row_step * ld + col_step * N, x_wrap = ld - dim;
+    const long long y_step = row_step * drow + col_step * N, y_wrap = drow - dim;
+    for (int j = first + blockIdx.y; j <= last; j += gridDim.y) {
         const int p0 = max(start, j * a.page), rows = min(len, (j + 1) * a.page) - p0;
-        const int page = a.table[(size_t)slot * a.max_pages + j % (a.cap / a.page)];
-        if (page < 0 || page >= a.n_pages) continue;
-        const T* src = (const T*)a.x[which] + (long long)(c0 + p0 - start) * ld + (size_t)g * dim;
-        unsigned char* dst = a.pool[which] + ((size_t)page * a.page * a.nkv + g) * dim;
-        const size_t drow = (size_t)a.nkv * dim;
+        const T* src = (const T*)a.x[which] + (c0 + p0 - start + row0) * ld + (size_t)g * dim + col0 * N;
         uint4 u[PIECES];
-        float amax = 0.f;
         int r = row0, c = col0;
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-            u[i] = r < rows ? __ldg(reinterpret_cast<const uint4*>(src + r * ld) + c) : make_uint4(0, 0, 0, 0);
+            u[i] = r < rows ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
             r += row_step;
             c += col_step;
-            if (c >= per_row) { c -= per_row; ++r; }
+            src += x_step;
+            if (c >= per_row) {
+                c -= per_row;
+                ++r;
+                src += x_wrap;
+            }
         }
+        const int page = a.table[(size_t)slot * a.max_pages + j % (a.cap / a.page)];
+        if (page < 0 || page >= a.n_pages) continue;
+        float amax = 0.f;
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) amax = fmaxf(amax, piece_max(u[i], T{}));
         amax = block_max(amax, scratch);
@@ -169,9 +176,11 @@ __global__ void __launch_bounds__(CP_THREADS) store_pages_e4m3_kernel(const Stor
             }
             amax = block_max(amax, scratch);
         }
+        unsigned char* dst = a.pool[which] + ((size_t)page * a.page * a.nkv + g) * dim;
         const int r0 = p0 - j * a.page;
         const float inv = e4m3_inverse(settle_scale(amax, a.scale[which] + (size_t)page * a.nkv + g, r0, dst, drow, dim));
-        dst += r0 * drow;
+        const f32x2 inv2 = pack2(inv, inv);
+        dst += (r0 + row0) * drow + col0 * N;
         r = row0;
         c = col0;
 #pragma unroll
@@ -182,26 +191,32 @@ __global__ void __launch_bounds__(CP_THREADS) store_pages_e4m3_kernel(const Stor
                 unsigned w[N / 4];
 #pragma unroll
                 for (int e = 0; e < N / 4; ++e) {
-                    const float x0 = x[4 * e] * inv, x1 = x[4 * e + 1] * inv, x2 = x[4 * e + 2] * inv, x3 = x[4 * e + 3] * inv;
-                    w[e] = infinite ? e4m3_pair(x0, x1) | e4m3_pair(x2, x3) << 16
-                                    : e4m3_pair_finite(x0, x1) | e4m3_pair_finite(x2, x3) << 16;
+                    float x0, x1, x2, x3;
+                    unpack2(mul2(pack2(x[4 * e], x[4 * e + 1]), inv2), x0, x1);
+                    unpack2(mul2(pack2(x[4 * e + 2], x[4 * e + 3]), inv2), x2, x3);
+                    w[e] = e4m3_pair_finite(x0, x1) | e4m3_pair_finite(x2, x3) << 16;
+                    if (infinite) w[e] = e4m3_pair(x0, x1) | e4m3_pair(x2, x3) << 16;
                 }
-                unsigned* to = reinterpret_cast<unsigned*>(dst + r * drow) + c * (N / 4);
-                if constexpr (N == 8) *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
-                else *to = w[0];
+                if constexpr (N == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+                else *reinterpret_cast<unsigned*>(dst) = w[0];
             }
             r += row_step;
             c += col_step;
-            if (c >= per_row) { c -= per_row; ++r; }
+            dst += y_step;
+            if (c >= per_row) {
+                c -= per_row;
+                ++r;
+                dst += y_wrap;
+            }
         }
     }
 }
 template <typename T>
 void launch_pages(const StoreE4& a, dim3 grid, int dim, cudaStream_t stream) {
-    constexpr int ALL = 64 * 256 * sizeof(T) / 16 / CP_THREADS;      // pieces of the greatest page: 8 or 16
-    if (dim > 128) agv_launch(store_pages_e4m3_kernel<T, ALL>, grid, CP_THREADS, 0, stream, a);
-    else if (dim > 64) agv_launch(store_pages_e4m3_kernel<T, ALL / 2>, grid, CP_THREADS, 0, stream, a);
-    else agv_launch(store_pages_e4m3_kernel<T, ALL / 4>, grid, CP_THREADS, 0, stream, a);
+    constexpr int THREADS = 128 * sizeof(T);                     // 8 pieces a thread in the greatest page
+    if (dim > 128) agv_launch(store_pages_e4m3_kernel<T, 8, THREADS>, grid, THREADS, 0, stream, a);
+    else if (dim > 64) agv_launch(store_pages_e4m3_kernel<T, 4, THREADS>, grid, THREADS, 0, stream, a);
+    else agv_launch(store_pages_e4m3_kernel<T, 2, THREADS>, grid, THREADS, 0, stream, a);
 }
 
 }  // namespace
@@ -230,7 +245,7 @@ AGV_API int agv_cache_store_e4m3(const void* k, long long ldk, const void* v, lo
     const int most = max_new < 1 ? 1 : max_new > T ? T : max_new;
     int blocks = most == 1 ? 1 : (most + page - 2) / page + 1;
     if (blocks > cap / page) blocks = cap / page;
-    const dim3 grid(blocks, 2 * nkv, B);
+    const dim3 grid(2 * nkv, blocks < 65535 ? blocks : 65535, B);
     const size_t esz = dtype == AGV_F32 ? 4 : 2;
     const int most_dim = hd > hdv ? hd : hdv;
     if (most > 1 && page <= 64 && most_dim <= 256 && agv_aligned(k, 16) && agv_aligned(v, 16) && ldk * esz % 16 == 0 &&

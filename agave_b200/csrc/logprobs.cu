@@ -6,7 +6,7 @@
 // reference c' as s' = s e^(c - c'), t' = (t + (c - c') s) e^(c - c').  (x - c comes before the factor
 // log2 e of the exponential: logits may be the type's lowest value.)
 //
-// What bounds it is reading the logits once.  A row is the work of a cluster of 1 to 16 CTAs; a
+// What bounds it is reading the logits once.  A row is the work of a cluster of 1 to 8 CTAs; a
 // thread takes every LP_THREADS-th 16 bytes of its CTA's slice, four of them while the next four are
 // under way, and keeps a running maximum, the two sums and the count of logits ahead of the
 // token's; the arithmetic goes two values an instruction where there is one for two.
@@ -21,12 +21,9 @@
 
 namespace {
 
-constexpr int LP_THREADS = 512;
-constexpr int LP_WARPS = LP_THREADS / 32;
 constexpr int LP_MAX_TOP = 32;
-constexpr int LP_MAX_CLUSTER = 16;
+constexpr int LP_MAX_CLUSTER = 8;
 constexpr int LP_GROUPS = 64;
-constexpr int LP_GROUP_LANES = LP_THREADS / LP_GROUPS;
 constexpr int LP_LIST = 2048;             // keys at or above the bound that a CTA can list
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -161,8 +158,9 @@ template <> struct Piece<__nv_bfloat16> {
 };
 __device__ __forceinline__ uint4 piece_at(const void* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
 
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(LP_THREADS, 2) logprobs_kernel(const Logprobs a) {
+template <typename T, bool TOP, int LP_THREADS>
+__global__ void __launch_bounds__(LP_THREADS, 1024 / LP_THREADS) logprobs_kernel(const Logprobs a) {
+    constexpr int LP_WARPS = LP_THREADS / 32, LP_GROUP_LANES = LP_THREADS / LP_GROUPS;
     constexpr int N = Piece<T>::N, BATCH = 4;
     __shared__ Sums wsum[LP_WARPS];
     __shared__ int wahead[LP_WARPS];
@@ -190,10 +188,10 @@ __global__ void __launch_bounds__(LP_THREADS, 2) logprobs_kernel(const Logprobs 
     uint4 next[BATCH];
     auto fetch = [&]() {
 #pragma unroll
-        for (int q = 0; q < BATCH; ++q) next[q] = piece_at(body + (size_t)(v + q * LP_THREADS) * N);
+        for (int q = 0; q < BATCH; ++q)
+            if (v + q * LP_THREADS < v1) next[q] = piece_at(body + (size_t)(v + q * LP_THREADS) * N);
     };
-    bool full = v + (BATCH - 1) * LP_THREADS < v1;
-    if (full) fetch();                                     // (before the token's logit is asked for)
+    fetch();                                               // (before the token's logit is asked for)
     const int tok = a.tokens[row];
     const bool has = tok >= 0 && tok < a.V;
     const float xt = has ? to_f32(x[tok]) : INFINITY;
@@ -256,19 +254,20 @@ __global__ void __launch_bounds__(LP_THREADS, 2) logprobs_kernel(const Logprobs 
             }
         }
     };
-    while (full) {
+    while (v < v1) {
         uint4 u[BATCH];
 #pragma unroll
         for (int q = 0; q < BATCH; ++q) u[q] = next[q];
-        const int i = head + v * N;
+        const int i = head + v * N, left = v1 - v;
         v += BATCH * LP_THREADS;
-        full = v + (BATCH - 1) * LP_THREADS < v1;
-        if (full) fetch();
-        take(u, std::integral_constant<int, BATCH>{}, i);
-    }
-    for (; v < v1; v += LP_THREADS) {
-        const uint4 u = piece_at(body + (size_t)v * N);
-        take(&u, std::integral_constant<int, 1>{}, head + v * N);
+        fetch();
+        if (left > (BATCH - 1) * LP_THREADS) {
+            take(u, std::integral_constant<int, BATCH>{}, i);
+        } else {
+#pragma unroll
+            for (int q = 0; q < BATCH - 1; ++q)
+                if (q * LP_THREADS < left) take(u + q, std::integral_constant<int, 1>{}, i + q * LP_THREADS * N);
+        }
     }
     // the head and what is left behind the last piece: a thread of the first CTA each
     const int tail = a.V - head - pieces * N;
@@ -445,31 +444,30 @@ __global__ void __launch_bounds__(LP_THREADS, 2) logprobs_kernel(const Logprobs 
     }
 }
 
-// CTAs for a row: the least of (rounds of CTAs) x (a slice's time and what a CTA costs besides).
-int lp_cluster(int R, int V, size_t esz) {
-    int best = 1;
-    double least = 1e30;
-    for (int C = 1; C <= LP_MAX_CLUSTER; C *= 2) {
-        if (C > 1 && V < C * 2048) break;                  // a slice of some thousand logits at least
-        const long long ctas = (long long)R * C;
-        const double rounds = (double)((ctas + 295) / 296);
-        const double us = rounds * (V * (double)esz / C / 22e3 + 3.0);
-        if (us < least) {
-            least = us;
-            best = C;
-        }
-    }
-    return best;
+// CTAs for a row: as many, up to 8, as leave slices of some thousand logits and at most about the 296 CTAs
+// of 512 threads that run at a time (64 rows of 262144: 35 us with one CTA a row, 23 with two, 22
+// with four, 35 with eight; one row: 27, 18, 13, 11; 64 rows of 32001: 9.2, 8.7, 10.3, 19).
+int lp_cluster(int R, int V) {
+    int C = 1;
+    while (C < 8 && (long long)R * C * 2 <= 296 && V >= C * 2 * 8000) C *= 2;
+    return C;
 }
 
-template <typename T, bool TOP>
+template <typename T, bool TOP, int THREADS>
 int lp_launch(const Logprobs& a, int R, cudaStream_t stream) {
-    auto kern = logprobs_kernel<T, TOP>;
-    if (a.cluster > 8)
-        AGV_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    agv_launch_cluster(kern, dim3((unsigned)(R * a.cluster)), LP_THREADS, 0, stream, dim3(a.cluster), a);
+    auto kern = logprobs_kernel<T, TOP, THREADS>;
+    agv_launch_cluster(kern, dim3((unsigned)(R * a.cluster)), THREADS, 0, stream, dim3(a.cluster), a);
     AGV_LAUNCH_OK("logprobs_kernel");
     return 0;
+}
+template <typename T>
+int lp_launch(const Logprobs& a, int R, cudaStream_t stream) {
+    // CTAs of 256 threads where there are several short rows for every SM: what a CTA does besides
+    // reading then runs under the others' reads (777 bfloat16 rows of 32001 31 us, 37 with 512
+    // threads; but 600 rows of 100000 65, and 59).
+    const bool small = (long long)R * a.cluster > 296 && a.V <= 65536;
+    if (a.top) return small ? lp_launch<T, true, 256>(a, R, stream) : lp_launch<T, true, 512>(a, R, stream);
+    return small ? lp_launch<T, false, 256>(a, R, stream) : lp_launch<T, false, 512>(a, R, stream);
 }
 
 }  // namespace
@@ -485,9 +483,8 @@ AGV_API int agv_token_logprobs(const void* logits, long long ld, int dtype, int 
                 V < LP_MAX_TOP ? V : LP_MAX_TOP);
     AGV_REQUIRE(dtype == AGV_F32 || dtype == AGV_BF16, "token_logprobs: bad dtype");
     if (R == 0) return 0;
-    const int C = lp_cluster(R, V, dtype == AGV_F32 ? 4 : 2);
+    const int C = lp_cluster(R, V);
     AGV_REQUIRE((long long)R * C <= 0x7fffffffLL, "token_logprobs: %d rows exceed the grid", R);
     Logprobs a{logits, ld, V, top, C, tokens, logprob, entropy, rank, top_ids, top_logprobs};
-    if (dtype == AGV_F32) return top ? lp_launch<float, true>(a, R, stream) : lp_launch<float, false>(a, R, stream);
-    return top ? lp_launch<__nv_bfloat16, true>(a, R, stream) : lp_launch<__nv_bfloat16, false>(a, R, stream);
+    return dtype == AGV_F32 ? lp_launch<float>(a, R, stream) : lp_launch<__nv_bfloat16>(a, R, stream);
 }
