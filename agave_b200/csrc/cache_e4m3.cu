@@ -10,6 +10,7 @@
 // rounding, read 16 bytes at a time.  Single tokens, and rows that do not start on 16 bytes, go two values
 // at a time and are read twice (the second time from L1); there it is the launch that counts.
 #include "e4m3.cuh"
+#include <type_traits>
 
 namespace {
 
@@ -116,13 +117,15 @@ __device__ __forceinline__ void piece_values(const uint4& u, float (&x)[16 / siz
     }
 }
 // (an infinity saturates here: for values that are known to have none)
-__device__ __forceinline__ unsigned e4m3_pair_finite(float a, float b) {
-    unsigned short r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
+__device__ __forceinline__ unsigned e4m3_quad_finite(float a, float b, float c, float d) {
+    unsigned r;
+    asm("{.reg .b16 l, h;\n cvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n cvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n"
+        " mov.b32 %0, {l, h};}" : "=r"(r) : "f"(a), "f"(b), "f"(c), "f"(d));
     return r;
 }
 
-template <typename T, int PIECES, int THREADS>
+// WHOLE: the pieces of a row are a power of two, so a thread's pieces are all in one column.
+template <typename T, int PIECES, int THREADS, bool WHOLE>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) store_pages_e4m3_kernel(const StoreE4 a) {
     constexpr int N = 16 / sizeof(T);
     pdl_wait();
@@ -137,10 +140,17 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) store_pages_e4m3_kern
     const int dim = a.dim[which], per_row = dim / N;
     // this thread's pieces, THREADS apart in the order of rows: the first one's row and column, and
     // the steps to the next
-    const int row0 = tid / per_row, col0 = tid % per_row, row_step = THREADS / per_row, col_step = THREADS % per_row;
+    int row0, col0, row_step, col_step;
+    if (WHOLE) {
+        const int bits = __ffs(per_row) - 1;
+        row0 = tid >> bits, col0 = tid & (per_row - 1), row_step = THREADS >> bits, col_step = 0;
+    } else {
+        row0 = tid / per_row, col0 = tid % per_row, row_step = THREADS / per_row, col_step = THREADS % per_row;
+    }
     const long long ld = a.ld[which], drow = (long long)a.nkv * dim;
+    // (a page of codes, and so the steps in it, are within 32 bits)
     const long long x_step = row_step * ld + col_step * N, x_wrap = ld - dim;
-    const long long y_step = row_step * drow + col_step * N, y_wrap = drow - dim;
+    const int y_step = row_step * (int)drow + col_step * N, y_wrap = (int)drow - dim;
     for (int j = first + blockIdx.y; j <= last; j += gridDim.y) {
         const int p0 = max(start, j * a.page), rows = min(len, (j + 1) * a.page) - p0;
         const T* src = (const T*)a.x[which] + (c0 + p0 - start + row0) * ld + (size_t)g * dim + col0 * N;
@@ -152,7 +162,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) store_pages_e4m3_kern
             r += row_step;
             c += col_step;
             src += x_step;
-            if (c >= per_row) {
+            if (!WHOLE && c >= per_row) {
                 c -= per_row;
                 ++r;
                 src += x_wrap;
@@ -183,40 +193,48 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) store_pages_e4m3_kern
         dst += (r0 + row0) * drow + col0 * N;
         r = row0;
         c = col0;
+        auto codes = [&](float x0, float x1, float x2, float x3, auto any) {
+            unpack2(mul2(pack2(x0, x1), inv2), x0, x1);
+            unpack2(mul2(pack2(x2, x3), inv2), x2, x3);
+            if constexpr (decltype(any)::value) return e4m3_pair(x0, x1) | e4m3_pair(x2, x3) << 16;
+            else return e4m3_quad_finite(x0, x1, x2, x3);
+        };
+        auto write = [&](auto any) {
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            if (r < rows) {
-                float x[N];
-                piece_values<T>(u[i], x);
-                unsigned w[N / 4];
-#pragma unroll
-                for (int e = 0; e < N / 4; ++e) {
-                    float x0, x1, x2, x3;
-                    unpack2(mul2(pack2(x[4 * e], x[4 * e + 1]), inv2), x0, x1);
-                    unpack2(mul2(pack2(x[4 * e + 2], x[4 * e + 3]), inv2), x2, x3);
-                    w[e] = e4m3_pair_finite(x0, x1) | e4m3_pair_finite(x2, x3) << 16;
-                    if (infinite) w[e] = e4m3_pair(x0, x1) | e4m3_pair(x2, x3) << 16;
+            for (int i = 0; i < PIECES; ++i) {
+                if (r < rows) {
+                    float x[N];
+                    piece_values<T>(u[i], x);
+                    const unsigned w = codes(x[0], x[1], x[2], x[3], any);
+                    if constexpr (N == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w, codes(x[N - 4], x[N - 3], x[N - 2], x[N - 1], any));
+                    else *reinterpret_cast<unsigned*>(dst) = w;
                 }
-                if constexpr (N == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
-                else *reinterpret_cast<unsigned*>(dst) = w[0];
+                r += row_step;
+                c += col_step;
+                dst += y_step;
+                if (!WHOLE && c >= per_row) {
+                    c -= per_row;
+                    ++r;
+                    dst += y_wrap;
+                }
             }
-            r += row_step;
-            c += col_step;
-            dst += y_step;
-            if (c >= per_row) {
-                c -= per_row;
-                ++r;
-                dst += y_wrap;
-            }
-        }
+        };
+        if (infinite) write(std::true_type{});
+        else write(std::false_type{});
     }
 }
-template <typename T>
-void launch_pages(const StoreE4& a, dim3 grid, int dim, cudaStream_t stream) {
+template <typename T, bool WHOLE>
+void launch_pages(const StoreE4& a, dim3 grid, cudaStream_t stream) {
     constexpr int THREADS = 128 * sizeof(T);                     // 8 pieces a thread in the greatest page
-    if (dim > 128) agv_launch(store_pages_e4m3_kernel<T, 8, THREADS>, grid, THREADS, 0, stream, a);
-    else if (dim > 64) agv_launch(store_pages_e4m3_kernel<T, 4, THREADS>, grid, THREADS, 0, stream, a);
-    else agv_launch(store_pages_e4m3_kernel<T, 2, THREADS>, grid, THREADS, 0, stream, a);
+    const int dim = a.dim[0] > a.dim[1] ? a.dim[0] : a.dim[1];
+    if (dim > 128) agv_launch(store_pages_e4m3_kernel<T, 8, THREADS, WHOLE>, grid, THREADS, 0, stream, a);
+    else if (dim > 64) agv_launch(store_pages_e4m3_kernel<T, 4, THREADS, WHOLE>, grid, THREADS, 0, stream, a);
+    else agv_launch(store_pages_e4m3_kernel<T, 2, THREADS, WHOLE>, grid, THREADS, 0, stream, a);
+}
+template <typename T>
+void launch_pages(const StoreE4& a, dim3 grid, cudaStream_t stream) {
+    if ((a.dim[0] & (a.dim[0] - 1)) == 0 && (a.dim[1] & (a.dim[1] - 1)) == 0) launch_pages<T, true>(a, grid, stream);
+    else launch_pages<T, false>(a, grid, stream);
 }
 
 }  // namespace
@@ -248,10 +266,10 @@ AGV_API int agv_cache_store_e4m3(const void* k, long long ldk, const void* v, lo
     const dim3 grid(2 * nkv, blocks < 65535 ? blocks : 65535, B);
     const size_t esz = dtype == AGV_F32 ? 4 : 2;
     const int most_dim = hd > hdv ? hd : hdv;
-    if (most > 1 && page <= 64 && most_dim <= 256 && agv_aligned(k, 16) && agv_aligned(v, 16) && ldk * esz % 16 == 0 &&
+    if (most > 1 && page <= 64 && most_dim <= 256 && (long long)page * nkv * most_dim <= 0x7fffffff && agv_aligned(k, 16) && agv_aligned(v, 16) && ldk * esz % 16 == 0 &&
         ldv * esz % 16 == 0) {
-        if (dtype == AGV_F32) launch_pages<float>(a, grid, most_dim, stream);
-        else launch_pages<__nv_bfloat16>(a, grid, most_dim, stream);
+        if (dtype == AGV_F32) launch_pages<float>(a, grid, stream);
+        else launch_pages<__nv_bfloat16>(a, grid, stream);
         AGV_LAUNCH_OK("store_pages_e4m3_kernel");
         return 0;
     }

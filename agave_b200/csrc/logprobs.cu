@@ -136,6 +136,20 @@ template <> struct Piece<float> {
         x[0] = __uint_as_float(u.x); x[1] = __uint_as_float(u.y);
         x[2] = __uint_as_float(u.z); x[3] = __uint_as_float(u.w);
     }
+    // (the pieces' sums below: what a value under -1e37 adds is 0 where ``tame`` is asked for)
+    static __device__ __forceinline__ uint4 tame(const uint4& u) { return u; }
+    static constexpr bool TAMES = false;
+    // values above, or at or above, the bound
+    static __device__ __forceinline__ f32x2 above(const uint4& u, float than, bool or_equal) {
+        const float x[4] = {__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w)};
+        float n[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (or_equal) asm("set.ge.f32.f32 %0, %1, %2;" : "=f"(n[i]) : "f"(x[i]), "f"(than));
+            else asm("set.gt.f32.f32 %0, %1, %2;" : "=f"(n[i]) : "f"(x[i]), "f"(than));
+        }
+        return add2(pack2(n[0], n[1]), pack2(n[2], n[3]));
+    }
     static __device__ __forceinline__ float greatest(const uint4& u) {
         return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
     }
@@ -149,6 +163,22 @@ template <> struct Piece<__nv_bfloat16> {
             x[2 * i] = __uint_as_float(w[i] << 16);
             x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
         }
+    }
+    static constexpr bool TAMES = true;
+    static __device__ __forceinline__ unsigned at_least(unsigned w) {
+        unsigned r;
+        asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0xfcf1fcf1u));       // -1e37 twice
+        return r;
+    }
+    static __device__ __forceinline__ uint4 tame(const uint4& u) {
+        return make_uint4(at_least(u.x), at_least(u.y), at_least(u.z), at_least(u.w));
+    }
+    static __device__ __forceinline__ f32x2 above(const uint4& u, float than, bool or_equal) {
+        const __nv_bfloat162 b = __float2bfloat162_rn(than);      // (a logit's own value: exact)
+        __nv_bfloat162 n;
+        if (or_equal) n = __hadd2(__hadd2(__hge2(pair(u.x), b), __hge2(pair(u.y), b)), __hadd2(__hge2(pair(u.z), b), __hge2(pair(u.w), b)));
+        else n = __hadd2(__hadd2(__hgt2(pair(u.x), b), __hgt2(pair(u.y), b)), __hadd2(__hgt2(pair(u.z), b), __hgt2(pair(u.w), b)));
+        return pack2(__low2float(n), __high2float(n));
     }
     static __device__ __forceinline__ __nv_bfloat162 pair(unsigned w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); }
     static __device__ __forceinline__ float greatest(const uint4& u) {
@@ -214,22 +244,31 @@ __global__ void __launch_bounds__(LP_THREADS, 1024 / LP_THREADS) logprobs_kernel
         const float c = sum.c == -INFINITY ? 0.f : sum.c;
         const f32x2 minus_c = pack2(-c, -c), log2e = pack2(LOG2E, LOG2E);
         f32x2 s = pack2(0.f, 0.f), w = pack2(0.f, 0.f);
+        auto add = [&](auto tame) {
 #pragma unroll
-        for (int q = 0; q < n; ++q) {
-            float x[N];
-            Piece<T>::values(u[q], x);
+            for (int q = 0; q < n; ++q) {
+                float x[N];
+                Piece<T>::values(decltype(tame)::value ? Piece<T>::tame(u[q]) : u[q], x);
 #pragma unroll
-            for (int e = 0; e < N; e += 2) {
-                // (at e^-150 a term is 0 and its product with d is, too)
-                float d0, d1, y0, y1;
-                unpack2(add2(pack2(x[e], x[e + 1]), minus_c), d0, d1);
-                const f32x2 d = pack2(max_nan(d0, -150.f), max_nan(d1, -150.f));
-                unpack2(mul2(d, log2e), y0, y1);
-                const f32x2 p = pack2(lp_ex2(y0), lp_ex2(y1));
-                s = add2(s, p);
-                w = fma2(p, d, w);
+                for (int e = 0; e < N; e += 2) {
+                    f32x2 d = add2(pack2(x[e], x[e + 1]), minus_c);
+                    float y0, y1;
+                    if constexpr (!decltype(tame)::value) {
+                        // (at e^-150 a term is 0 and its product with d is, too)
+                        unpack2(d, y0, y1);
+                        d = pack2(max_nan(y0, -150.f), max_nan(y1, -150.f));
+                    }
+                    unpack2(mul2(d, log2e), y0, y1);
+                    const f32x2 p = pack2(lp_ex2(y0), lp_ex2(y1));
+                    s = add2(s, p);
+                    w = fma2(p, d, w);
+                }
             }
-        }
+        };
+        // Where the reference is no extreme number, bfloat16 values are held above -1e37, two an
+        // instruction: d is then finite, and such a value's term 0 as ever.
+        if (Piece<T>::TAMES && fabsf(c) < 1e30f) add(std::integral_constant<bool, Piece<T>::TAMES>{});
+        else add(std::false_type{});
         float lo, hi;
         unpack2(s, lo, hi);
         sum.s += lo + hi;
@@ -237,17 +276,22 @@ __global__ void __launch_bounds__(LP_THREADS, 1024 / LP_THREADS) logprobs_kernel
         sum.t += lo + hi;
         if (bm >= xt) {
             const int end = i + (n - 1) * LP_THREADS * N + N;
-#pragma unroll
-            for (int q = 0; q < n; ++q) {
-                float x[N];
-                Piece<T>::values(u[q], x);
+            if (i > tok || end <= tok) {
+                f32x2 count = pack2(0.f, 0.f);
                 if (i > tok) {
 #pragma unroll
-                    for (int e = 0; e < N; ++e) ahead += x[e] > xt;
-                } else if (end <= tok) {
-#pragma unroll
-                    for (int e = 0; e < N; ++e) ahead += x[e] >= xt;
+                    for (int q = 0; q < n; ++q) count = add2(count, Piece<T>::above(u[q], xt, false));
                 } else {
+#pragma unroll
+                    for (int q = 0; q < n; ++q) count = add2(count, Piece<T>::above(u[q], xt, true));
+                }
+                unpack2(count, lo, hi);
+                ahead += (int)(lo + hi);
+            } else {
+#pragma unroll
+                for (int q = 0; q < n; ++q) {
+                    float x[N];
+                    Piece<T>::values(u[q], x);
 #pragma unroll
                     for (int e = 0; e < N; ++e) ahead += x[e] > xt || (x[e] == xt && i + q * LP_THREADS * N + e < tok);
                 }
