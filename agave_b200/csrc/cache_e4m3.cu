@@ -23,7 +23,7 @@ struct StoreE4 {
     float* scale[2];               // [pages, nkv]
     int dim[2];
     const int *cu, *slots, *lens, *table;
-    int T, n_slots, max_pages, n_pages, page, cap, nkv;
+    int T, n_slots, max_pages, n_pages, page_bits, ring, nkv;      // a sequence's pages: a ring of so many
 };
 
 // Scale of a page and head from the new rows' magnitude and, where the page goes on (r0 rows of it
@@ -55,19 +55,19 @@ __global__ void __launch_bounds__(CE_THREADS) store_e4m3_kernel(const StoreE4 a)
     pdl_launch_next();
     __shared__ float scratch[32];
     // (the heads of a page beside each other on the grid: together their rows are whole)
-    const int b = blockIdx.z, which = blockIdx.x / a.nkv, g = blockIdx.x % a.nkv, tid = threadIdx.x;
+    const int b = blockIdx.z >> 1, which = blockIdx.z & 1, g = blockIdx.x, tid = threadIdx.x;
     const int slot = a.slots[b], c0 = a.cu[b], n = a.cu[b + 1] - c0, len = a.lens[b];
     if (slot < 0 || slot >= a.n_slots || n <= 0 || c0 < 0 || c0 > a.T - n || len < n) return;
-    const int start = len - n, last = (len - 1) / a.page;
-    const int first = max(start / a.page, last - a.cap / a.page + 1);
+    const int start = len - n, last = (len - 1) >> a.page_bits;
+    const int first = max(start >> a.page_bits, last - a.ring + 1);
     const int dim = a.dim[which];
     const T* x = (const T*)a.x[which] + (size_t)g * dim;
     for (int j = first + blockIdx.y; j <= last; j += gridDim.y) {
-        const int p0 = max(start, j * a.page), p1 = min(len, (j + 1) * a.page);
-        const int page = a.table[(size_t)slot * a.max_pages + j % (a.cap / a.page)];
+        const int p0 = max(start, j << a.page_bits), p1 = min(len, (j + 1) << a.page_bits);
+        const int page = a.table[(size_t)slot * a.max_pages + (j < a.ring ? j : j % a.ring)];
         if (page < 0 || page >= a.n_pages) continue;
         const T* src = x + (long long)(c0 + p0 - start) * a.ld[which];
-        unsigned char* dst = a.pool[which] + (((size_t)page * a.page) * a.nkv + g) * dim;
+        unsigned char* dst = a.pool[which] + (((size_t)page << a.page_bits) * a.nkv + g) * dim;
         float* sc = a.scale[which] + (size_t)page * a.nkv + g;
         const int pairs = (p1 - p0) * dim / 2, half = dim / 2;
         float amax = 0.f;
@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(CE_THREADS) store_e4m3_kernel(const StoreE4 a)
             amax = fmaxf(amax, fmaxf(e4m3_magnitude(to_f32(e[0])), e4m3_magnitude(to_f32(e[1]))));
         }
         amax = block_max(amax, scratch);
-        const int r0 = p0 - j * a.page;
+        const int r0 = p0 - (j << a.page_bits);
         const float s = settle_scale(amax, sc, r0, dst, (size_t)a.nkv * dim, dim);
         const float inv = e4m3_inverse(s);
         for (int i = tid; i < pairs; i += CE_THREADS) {
@@ -126,17 +126,17 @@ __device__ __forceinline__ unsigned e4m3_quad_finite(float a, float b, float c, 
 
 // WHOLE: the pieces of a row are a power of two, so a thread's pieces are all in one column.
 template <typename T, int PIECES, int THREADS, bool WHOLE>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) store_pages_e4m3_kernel(const StoreE4 a) {
+__global__ void __launch_bounds__(THREADS, (WHOLE || THREADS > 256 ? 1024 : 768) / THREADS) store_pages_e4m3_kernel(const StoreE4 a) {
     constexpr int N = 16 / sizeof(T);
     pdl_wait();
     pdl_launch_next();
     __shared__ float scratch[32];
     // (the heads of a page beside each other on the grid: together their rows are whole)
-    const int b = blockIdx.z, which = blockIdx.x / a.nkv, g = blockIdx.x % a.nkv, tid = threadIdx.x;
+    const int b = blockIdx.z >> 1, which = blockIdx.z & 1, g = blockIdx.x, tid = threadIdx.x;
     const int slot = a.slots[b], c0 = a.cu[b], n = a.cu[b + 1] - c0, len = a.lens[b];
     if (slot < 0 || slot >= a.n_slots || n <= 0 || c0 < 0 || c0 > a.T - n || len < n) return;
-    const int start = len - n, last = (len - 1) / a.page;
-    const int first = max(start / a.page, last - a.cap / a.page + 1);
+    const int start = len - n, last = (len - 1) >> a.page_bits;
+    const int first = max(start >> a.page_bits, last - a.ring + 1);
     const int dim = a.dim[which], per_row = dim / N;
     // this thread's pieces, THREADS apart in the order of rows: the first one's row and column, and
     // the steps to the next
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) store_pages_e4m3_kern
     const long long x_step = row_step * ld + col_step * N, x_wrap = ld - dim;
     const int y_step = row_step * (int)drow + col_step * N, y_wrap = (int)drow - dim;
     for (int j = first + blockIdx.y; j <= last; j += gridDim.y) {
-        const int p0 = max(start, j * a.page), rows = min(len, (j + 1) * a.page) - p0;
+        const int p0 = max(start, j << a.page_bits), rows = min(len, (j + 1) << a.page_bits) - p0;
         const T* src = (const T*)a.x[which] + (c0 + p0 - start + row0) * ld + (size_t)g * dim + col0 * N;
         uint4 u[PIECES];
         int r = row0, c = col0;
@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) store_pages_e4m3_kern
                 src += x_wrap;
             }
         }
-        const int page = a.table[(size_t)slot * a.max_pages + j % (a.cap / a.page)];
+        const int page = a.table[(size_t)slot * a.max_pages + (j < a.ring ? j : j % a.ring)];
         if (page < 0 || page >= a.n_pages) continue;
         float amax = 0.f;
 #pragma unroll
@@ -186,8 +186,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) store_pages_e4m3_kern
             }
             amax = block_max(amax, scratch);
         }
-        unsigned char* dst = a.pool[which] + ((size_t)page * a.page * a.nkv + g) * dim;
-        const int r0 = p0 - j * a.page;
+        unsigned char* dst = a.pool[which] + (((size_t)page << a.page_bits) * a.nkv + g) * dim;
+        const int r0 = p0 - (j << a.page_bits);
         const float inv = e4m3_inverse(settle_scale(amax, a.scale[which] + (size_t)page * a.nkv + g, r0, dst, drow, dim));
         const f32x2 inv2 = pack2(inv, inv);
         dst += (r0 + row0) * drow + col0 * N;
@@ -252,18 +252,20 @@ AGV_API int agv_cache_store_e4m3(const void* k, long long ldk, const void* v, lo
     AGV_REQUIRE(B >= 0 && T >= 0 && nkv > 0 && n_slots > 0 && n_pages > 0, "cache_store_e4m3: bad sizes");
     AGV_REQUIRE(hd > 0 && hd % 16 == 0 && hdv > 0 && hdv % 16 == 0,
                 "cache_store_e4m3: head sizes %d and %d must be multiples of 16", hd, hdv);
-    AGV_REQUIRE(page > 0 && cap > 0 && cap % page == 0 && cap / page <= max_pages,
+    AGV_REQUIRE(page > 0 && (page & (page - 1)) == 0 && cap > 0 && cap % page == 0 && cap / page <= max_pages,
                 "cache_store_e4m3: bad cache geometry (page %d, cap %d, table of %d)", page, cap, max_pages);
     AGV_REQUIRE(dtype == AGV_F32 || dtype == AGV_BF16, "cache_store_e4m3: bad dtype");
     AGV_REQUIRE(agv_aligned(k_pool, 16) && agv_aligned(v_pool, 16), "cache_store_e4m3: unaligned pool");
-    AGV_REQUIRE(B <= 65535 && nkv <= 32767, "cache_store_e4m3: %d sequences, %d heads exceed the grid", B, nkv);
+    AGV_REQUIRE(B <= 32767, "cache_store_e4m3: %d sequences exceed the grid", B);
     if (B == 0 || T == 0) return 0;
+    int page_bits = 0;
+    while (1 << page_bits < page) ++page_bits;
     StoreE4 a{{k, v}, {ldk, ldv}, {(unsigned char*)k_pool, (unsigned char*)v_pool}, {k_scale, v_scale},
-              {hd, hdv}, cu, slots, lens, table, T, n_slots, max_pages, n_pages, page, cap, nkv};
+              {hd, hdv}, cu, slots, lens, table, T, n_slots, max_pages, n_pages, page_bits, cap / page, nkv};
     const int most = max_new < 1 ? 1 : max_new > T ? T : max_new;
     int blocks = most == 1 ? 1 : (most + page - 2) / page + 1;
     if (blocks > cap / page) blocks = cap / page;
-    const dim3 grid(2 * nkv, blocks < 65535 ? blocks : 65535, B);
+    const dim3 grid(nkv, blocks < 65535 ? blocks : 65535, 2 * B);
     const size_t esz = dtype == AGV_F32 ? 4 : 2;
     const int most_dim = hd > hdv ? hd : hdv;
     if (most > 1 && page <= 64 && most_dim <= 256 && (long long)page * nkv * most_dim <= 0x7fffffff && agv_aligned(k, 16) && agv_aligned(v, 16) && ldk * esz % 16 == 0 &&

@@ -97,10 +97,12 @@ class _DecodeGraph:
         # before the result of the step before it has been read
         self.next_hosts = [torch.zeros(B, dtype=torch.int32, pin_memory=True) for _ in range(2)]
         self.done = [torch.cuda.Event() for _ in range(2)]
-        self.scores: Optional[kernels.TokenLogprobs] = None
+        self.scores: Optional[torch.Tensor] = None     # packed log-probabilities of the step
         self.score_hosts = [None, None]
         if top is not None:
-            self.score_hosts = [torch.zeros((3 + 2 * top) * B, pin_memory=True) for _ in range(2)]
+            n = kernels.token_logprobs_words(B, top)
+            self.scores = torch.zeros(n, dtype=torch.float32, device=dev)
+            self.score_hosts = [torch.zeros(n, pin_memory=True) for _ in range(2)]
         self.logits: Optional[torch.Tensor] = None
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.kernels_per_step = 0
@@ -130,7 +132,7 @@ class _DecodeGraph:
         engine.sampler.choose(self.logits, self.next_dev, params, seed, v["slots"], self.seq_ids,
                               v["steps"], penalise=True, dev_params=self.words)
         if self.top is not None:
-            self.scores = kernels.token_logprobs(raw, self.next_dev, self.top)
+            kernels.token_logprobs(raw, self.next_dev, self.top, packed=self.scores)
 
     def _record(self, engine: "Engine", params: SamplingParams, seed: int) -> None:
         if not engine.use_graphs:
@@ -170,7 +172,7 @@ class _DecodeGraph:
             self._body(engine, params, seed)
         self.next_hosts[which].copy_(self.next_dev, non_blocking=True)
         if self.top is not None:
-            self.score_hosts[which].copy_(self.scores.packed, non_blocking=True)
+            self.score_hosts[which].copy_(self.scores, non_blocking=True)
         self.done[which].record()
 
     def wait(self, which: int = 0) -> "np.ndarray":
@@ -180,7 +182,7 @@ class _DecodeGraph:
 
     def token_scores(self, which: int):
         """The log-probabilities that came with those tokens (after ``wait``)."""
-        return kernels.TokenLogprobs.unpack(self.score_hosts[which].numpy(), self.size, self.top)
+        return kernels.unpack_token_logprobs(self.score_hosts[which].numpy(), self.size, self.top)
 
     def run(self, engine: "Engine", params: SamplingParams, seed: int) -> None:
         self.launch(engine, params, seed)
@@ -378,11 +380,13 @@ class Engine:
                 at += n
             both = torch.tensor([rows, targets], dtype=torch.int32).to(self.device)
             step = max(1, SCORE_LOGITS // self.spec.vocab_size)
+            packed = torch.empty(kernels.token_logprobs_words(min(step, len(rows)), top),
+                                 dtype=torch.float32, device=self.device)
             for a in range(0, len(rows), step):
                 logits = self.model.logits(h, both[0, a:a + step], ctx)
-                found = kernels.token_logprobs(logits, both[1, a:a + step], top)
                 n = logits.shape[0]
-                host = kernels.TokenLogprobs.unpack(found.packed.cpu().numpy(), n, top)
+                kernels.token_logprobs(logits, both[1, a:a + step], top, packed=packed)
+                host = kernels.unpack_token_logprobs(packed.cpu().numpy(), n, top)
                 for i in range(n):
                     out[owners[a + i]].append(_score(targets[a + i], host, i))
         finally:
@@ -411,8 +415,10 @@ class Engine:
             found = None
             if top is not None:
                 # (the first choice is made without a penalty: the logits are as they were)
-                found = kernels.TokenLogprobs.unpack(
-                    kernels.token_logprobs(logits, first, top).packed.cpu().numpy(), B, top)
+                packed = torch.empty(kernels.token_logprobs_words(B, top), dtype=torch.float32,
+                                     device=dev)
+                kernels.token_logprobs(logits, first, top, packed=packed)
+                found = kernels.unpack_token_logprobs(packed.cpu().numpy(), B, top)
             stats["prefill_seconds"] += time.perf_counter() - t0
             stats["prefill_tokens"] += sum(len(r.prompt) for r in batch)
             ended = plan.accept({r.index: int(first_host[i]) for i, r in enumerate(batch)})

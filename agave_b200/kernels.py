@@ -110,6 +110,14 @@ def _span(op: str, nbytes: int = 0, flops: int = 0):
     return _perf.span(op, nbytes, flops)
 
 
+_UNWATCHED = _perf_mod.NULL_SPAN
+
+
+def _watched() -> bool:
+    """Whether launches are timed or named at all."""
+    return _perf is not None or NVTX
+
+
 def _nbytes(*tensors) -> int:
     return sum(t.numel() * t.element_size() for t in tensors if t is not None)
 
@@ -2101,7 +2109,8 @@ def cache_store_e4m3(k: torch.Tensor, v: torch.Tensor, view, ctx, n_kv_heads: in
     _require(cu.numel() == B + 1 and lens.numel() == B and cu.is_contiguous() and
              slots.is_contiguous() and lens.is_contiguous(),
              "cache_store_e4m3: cu_seqlens [B + 1], slots [B] and lens [B] do not fit")
-    with _span("cache_store", T * n_kv_heads * (head_dim + hdv) * (k.element_size() + 1)):
+    with _span("cache_store", T * n_kv_heads * (head_dim + hdv) * (k.element_size() + 1)) \
+            if _watched() else _UNWATCHED:
         _check(library().agv_cache_store_e4m3(
             k.data_ptr(), ldk, v.data_ptr(), ldv, dtype_code(k.dtype), cu.data_ptr(),
             slots.data_ptr(), lens.data_ptr(), B, T, int(ctx.max_new), n_kv_heads, head_dim, hdv,
@@ -2156,8 +2165,8 @@ def attention_decode_e4m3(q: torch.Tensor, out: torch.Tensor, view, ctx, n_heads
     if floats < 0:
         _check(floats)
     partial = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-    cost = _attention_cost(ctx, q, None, None, out, n_heads, head_dim, window, n_kv_heads, 1)
-    with _span(op, *cost):
+    with _span(op, *_attention_cost(ctx, q, None, None, out, n_heads, head_dim, window, n_kv_heads,
+                                    1)) if _watched() else _UNWATCHED:
         _check(lib.agv_attention_decode_e4m3(
             q.data_ptr(), q.stride(0), out.data_ptr(), dtype_code(q.dtype), kp.data_ptr(),
             vp.data_ptr(), ks.data_ptr(), vs.data_ptr(), table.data_ptr(), n_slots, max_pages,
@@ -2175,60 +2184,59 @@ LOGPROBS_MAX_TOP = 32
 class TokenLogprobs:
     """What ``token_logprobs`` finds for R rows: ``logprob`` and ``entropy`` [R] (32-bit, nats),
     ``rank`` [R] (int32; 1 = the greatest logit), ``top_ids`` [R, top] (int32) and
-    ``top_logprobs`` [R, top] (32-bit), greatest first, equal ones by index.  They are views of
-    ``packed``, 32 bits a value in this order, which one copy brings to the host (``unpack``)."""
-    __slots__ = ("packed", "rows", "top")
-
-    def __init__(self, packed: torch.Tensor, rows: int, top: int):
-        self.packed, self.rows, self.top = packed, rows, top
-
-    @property
-    def logprob(self) -> torch.Tensor:
-        return self.packed[:self.rows]
-
-    @property
-    def entropy(self) -> torch.Tensor:
-        return self.packed[self.rows:2 * self.rows]
-
-    @property
-    def rank(self) -> torch.Tensor:
-        return self.packed[2 * self.rows:3 * self.rows].view(torch.int32)
-
-    @property
-    def top_ids(self) -> torch.Tensor:
-        n = self.rows * self.top
-        return self.packed[3 * self.rows:3 * self.rows + n].view(torch.int32).view(self.rows, self.top)
-
-    @property
-    def top_logprobs(self) -> torch.Tensor:
-        return self.packed[(3 + self.top) * self.rows:].view(self.rows, self.top)
-
-    @staticmethod
-    def unpack(packed, rows: int, top: int):
-        """(logprob, entropy, rank, top ids, top logprobs) of a host copy of ``packed`` (numpy)."""
-        i = packed.view("int32")
-        ids, lps = i[3 * rows:(3 + top) * rows], packed[(3 + top) * rows:(3 + 2 * top) * rows]
-        return (packed[:rows], packed[rows:2 * rows], i[2 * rows:3 * rows], ids.reshape(rows, top),
-                lps.reshape(rows, top))
+    ``top_logprobs`` [R, top] (32-bit), greatest first, equal ones by index."""
+    __slots__ = ("logprob", "entropy", "rank", "top_ids", "top_logprobs")
 
 
-def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
+def token_logprobs_words(rows: int, top: int) -> int:
+    """32-bit values that ``token_logprobs`` writes for so many rows."""
+    return (3 + 2 * top) * rows
+
+
+def unpack_token_logprobs(packed, rows: int, top: int):
+    """(logprob, entropy, rank, top ids, top logprobs) of a host copy of ``packed`` (numpy)."""
+    i = packed.view("int32")
+    ids, lps = i[3 * rows:(3 + top) * rows], packed[(3 + top) * rows:(3 + 2 * top) * rows]
+    return (packed[:rows], packed[rows:2 * rows], i[2 * rows:3 * rows], ids.reshape(rows, top),
+            lps.reshape(rows, top))
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
+                   packed: Optional[torch.Tensor] = None) -> Optional[TokenLogprobs]:
     """ln softmax(logits[r])[tokens[r]] for every row of logits [R, V] (32-bit or bfloat16, rows
     may be strided), the row's entropy, the token's rank and the ``top`` (at most 32) greatest,
     from one pass over the logits.  A logit of -inf is a probability of zero.  A token outside
     the vocabulary stands for none: logprob NaN, rank 0.  Rows that have no softmax (NaN or +inf
-    in them, or nothing but -inf) give NaN; NaN stands below every number among the greatest."""
-    _on_current_device(logits, tokens)
+    in them, or nothing but -inf) give NaN; NaN stands below every number among the greatest.
+
+    ``packed`` (32-bit, ``token_logprobs_words`` values): everything goes there, one after the
+    other, so that one copy brings it to the host (``unpack_token_logprobs``), and None is
+    returned."""
+    _on_current_device(logits, tokens, packed)
     _require(logits.dim() == 2 and logits.stride(1) == 1, "token_logprobs: logits must be [rows, vocabulary]")
     R, V = logits.shape
     _i32(tokens, "tokens")
     _require(tokens.numel() == R and tokens.is_contiguous(), f"token_logprobs: one token for each of {R} rows")
-    _require(0 <= top <= V and top <= LOGPROBS_MAX_TOP,
-             f"token_logprobs: top {top} must lie in 0..{min(V, LOGPROBS_MAX_TOP)}")
-    packed = torch.empty((3 + 2 * top) * R, dtype=torch.float32, device=logits.device)
-    at, n = packed.data_ptr(), 4 * R
-    with _span("token_logprobs", _nbytes(logits, packed) if _perf is not None else 0):
+    if not (0 <= top <= V and top <= LOGPROBS_MAX_TOP):
+        raise KernelError(f"token_logprobs: top {top} must lie in 0..{min(V, LOGPROBS_MAX_TOP)}")
+    r = None
+    if packed is None:
+        r, new, i32, dev = TokenLogprobs(), torch.empty, torch.int32, logits.device
+        r.logprob = new(R, dtype=torch.float32, device=dev)
+        r.entropy = new(R, dtype=torch.float32, device=dev)
+        r.rank = new(R, dtype=i32, device=dev)
+        r.top_ids = new((R, top), dtype=i32, device=dev)
+        r.top_logprobs = new((R, top), dtype=torch.float32, device=dev)
+        out = (r.logprob.data_ptr(), r.entropy.data_ptr(), r.rank.data_ptr(), r.top_ids.data_ptr(),
+               r.top_logprobs.data_ptr())
+    else:
+        _f32(packed, "packed")
+        _require(packed.is_contiguous() and packed.numel() >= token_logprobs_words(R, top),
+                 f"token_logprobs: packed must hold {token_logprobs_words(R, top)} values")
+        at, n = packed.data_ptr(), 4 * R
+        out = (at, at + n, at + 2 * n, at + 3 * n, at + (3 + top) * n)
+    with _span("token_logprobs", _nbytes(logits)) if _watched() else _UNWATCHED:
         _check(library().agv_token_logprobs(
             logits.data_ptr(), logits.stride(0), dtype_code(logits.dtype), R, V, tokens.data_ptr(),
-            top, at, at + n, at + 2 * n, at + 3 * n, at + (3 + top) * n, _stream_handle()))
-    return TokenLogprobs(packed, R, top)
+            top, *out, _stream_handle()))
+    return r

@@ -138,6 +138,27 @@ def test_rows_without_a_softmax_and_tokens_outside():
     assert torch.equal(r.top_ids[1].long(), torch.sort(y, descending=True, stable=True).indices[:3])
 
 
+def same(a, b):
+    return all(torch.equal(getattr(a, n).view(torch.int32), getattr(b, n).view(torch.int32)) for n in a.__slots__)
+
+
+def test_packed_results():
+    from agave_b200 import kernels
+    g = torch.Generator().manual_seed(8)
+    for R, top in ((1, 0), (5, 3), (40, 32)):
+        x = (torch.randn(R, 5000, generator=g) * 3).to(DEV)
+        t = torch.randint(0, 5000, (R,), generator=g).int().to(DEV)
+        r = kernels.token_logprobs(x, t, top)
+        packed = torch.zeros(kernels.token_logprobs_words(R, top) + 5, device=DEV)
+        assert kernels.token_logprobs(x, t, top, packed=packed) is None
+        assert (packed[-5:] == 0).all()
+        for a, b in zip(kernels.unpack_token_logprobs(packed.cpu().numpy(), R, top),
+                        (r.logprob, r.entropy, r.rank, r.top_ids, r.top_logprobs)):
+            assert a.shape == b.shape and (a == b.cpu().numpy()).all()
+        with pytest.raises(kernels.KernelError, match="packed"):
+            kernels.token_logprobs(x, t, top, packed=packed[:2])
+
+
 def test_recorded_and_replayed_and_streams():
     """A recording follows its inputs, and calls on two streams do not share anything."""
     from agave_b200 import kernels
@@ -155,7 +176,7 @@ def test_recorded_and_replayed_and_streams():
         x.copy_(a); t.copy_(b)
         graph.replay()
         want = check(a, b, 7)
-        assert torch.equal(r.packed.view(torch.int32), want.packed.view(torch.int32))
+        assert same(r, want)
     streams = [torch.cuda.Stream() for _ in range(2)]
     torch.cuda.synchronize()
     got = [[], []]
@@ -167,7 +188,7 @@ def test_recorded_and_replayed_and_streams():
     for s in range(2):
         want = check(xs[s], ts[s], 7)
         for r in got[s]:
-            assert torch.equal(r.packed.view(torch.int32), want.packed.view(torch.int32))
+            assert same(r, want)
 
 
 def test_refusals():
