@@ -113,11 +113,6 @@ def _span(op: str, nbytes: int = 0, flops: int = 0):
 _UNWATCHED = _perf_mod.NULL_SPAN
 
 
-def _watched() -> bool:
-    """Whether launches are timed or named at all."""
-    return _perf is not None or NVTX
-
-
 def _nbytes(*tensors) -> int:
     return sum(t.numel() * t.element_size() for t in tensors if t is not None)
 
@@ -2059,25 +2054,54 @@ def e4m3_head_supported(head_dim: int, value_dim: int = 0) -> bool:
     return all(d % 16 == 0 and 0 < d <= E4M3_MAX_HEAD for d in (head_dim, value_dim or head_dim))
 
 
-def _e4m3_view(view, n_kv_heads: int, head_dim: int, value_dim: int, what: str):
-    """Checks a cache entry's pools, scales and table; (slots of the table, its width, pages)."""
+def _refuse_e4m3_view(view, n_kv_heads: int, head_dim: int, value_dim: int, what: str) -> None:
+    """Says what is wrong with a cache entry's pools, scales or table, if something is."""
     k, v, ks, vs, table = view.k_pool, view.v_pool, view.k_scale, view.v_scale, view.page_table
+    pages = k.shape[0]
     _require(k.dtype == E4M3 and v.dtype == E4M3, f"{what}: the pools must hold float8_e4m3fn codes")
-    shape = k.shape
-    pages = shape[0]
-    if shape != (pages, view.page, n_kv_heads, head_dim) or \
-            v.shape != (pages, view.page, n_kv_heads, value_dim):
-        raise KernelError(f"{what}: pools {tuple(shape)} and {tuple(v.shape)} are not [pages, "
-                          f"{view.page}, {n_kv_heads}, head size]")
-    if not (k.is_contiguous() and v.is_contiguous() and table.is_contiguous() and
-            ks.is_contiguous() and vs.is_contiguous()):
-        raise KernelError(f"{what}: pools, scales and page table must be contiguous")
-    if ks.dtype != torch.float32 or vs.dtype != torch.float32 or \
-            not (ks.shape == vs.shape == (pages, n_kv_heads)):
-        raise KernelError(f"{what}: scales must be float32 [{pages}, {n_kv_heads}]")
+    _require(k.shape == (pages, view.page, n_kv_heads, head_dim) and
+             v.shape == (pages, view.page, n_kv_heads, value_dim),
+             f"{what}: pools {tuple(k.shape)} and {tuple(v.shape)} are not [pages, {view.page}, "
+             f"{n_kv_heads}, head size]")
+    _require(k.is_contiguous() and v.is_contiguous() and table.is_contiguous() and
+             ks.is_contiguous() and vs.is_contiguous(),
+             f"{what}: pools, scales and page table must be contiguous")
+    _require(ks.dtype == torch.float32 and vs.dtype == torch.float32 and
+             ks.shape == vs.shape == (pages, n_kv_heads),
+             f"{what}: scales must be float32 [{pages}, {n_kv_heads}]")
     _i32(table, "page_table")
-    n_slots, max_pages = table.shape
-    return n_slots, max_pages, pages
+    _require(table.dim() == 2, f"{what}: the page table is [slots, pages of a slot]")
+
+
+def _refuse_store(k, v, view, ctx, n_kv_heads: int, head_dim: int, hdv: int) -> None:
+    """Says why ``cache_store_e4m3`` does not take its arguments (called where one of its checks,
+    which are made together, has failed)."""
+    cu, slots, lens = ctx.cu_seqlens, ctx.slots, ctx.lens
+    _on_current_device(k, v, view.k_pool, view.v_pool, view.k_scale, view.v_scale, view.page_table,
+                       cu, slots, lens)
+    _require(k.dim() == 2 and k.shape[1] == n_kv_heads * head_dim and
+             v.shape == (k.shape[0], n_kv_heads * hdv),
+             f"cache_store_e4m3: keys {tuple(k.shape)} and values {tuple(v.shape)} do not fit "
+             f"{n_kv_heads} heads of {head_dim} and {hdv}")
+    _require(k.dtype == v.dtype, f"cache_store_e4m3: keys {k.dtype} and values {v.dtype} differ")
+    _require(k.stride(1) == 1 and v.stride(1) == 1, "cache_store_e4m3: elements of a row must be adjacent")
+    _refuse_e4m3_view(view, n_kv_heads, head_dim, hdv, "cache_store_e4m3")
+    _i32(cu, "cu_seqlens"); _i32(slots, "slots"); _i32(lens, "lens")
+    raise KernelError("cache_store_e4m3: cu_seqlens [B + 1], slots [B] and lens [B] do not fit")
+
+
+def _refuse_attend(q, out, view, ctx, n_heads: int, n_kv_heads: int, head_dim: int, hdv: int) -> None:
+    """The same for ``attention_decode_e4m3``."""
+    slots, positions, B = ctx.slots, ctx.positions, q.shape[0]
+    _on_current_device(q, out, view.k_pool, view.v_pool, view.k_scale, view.v_scale,
+                       view.page_table, slots, positions)
+    _require(q.dim() == 2 and q.shape[1] == n_heads * head_dim and q.stride(1) == 1,
+             f"attention_decode_e4m3: queries {tuple(q.shape)} are not [B, {n_heads} * {head_dim}]")
+    _require(out.dtype == q.dtype and out.shape == (B, n_heads * hdv) and out.is_contiguous(),
+             f"attention_decode_e4m3: the output must be contiguous [{B}, {n_heads * hdv}] of {q.dtype}")
+    _refuse_e4m3_view(view, n_kv_heads, head_dim, hdv, "attention_decode_e4m3")
+    _i32(slots, "slots"); _i32(positions, "positions")
+    raise KernelError("attention_decode_e4m3: one slot and position per query")
 
 
 def cache_store_e4m3(k: torch.Tensor, v: torch.Tensor, view, ctx, n_kv_heads: int, head_dim: int,
@@ -2096,26 +2120,40 @@ def cache_store_e4m3(k: torch.Tensor, v: torch.Tensor, view, ctx, n_kv_heads: in
     hdv = value_dim or head_dim
     cu, slots, lens = ctx.cu_seqlens, ctx.slots, ctx.lens
     kp, vp, ks, vs, table = view.k_pool, view.v_pool, view.k_scale, view.v_scale, view.page_table
-    _on_current_device(k, v, kp, vp, ks, vs, table, cu, slots, lens)
-    T, B = k.shape[0], slots.numel()
-    if k.shape != (T, n_kv_heads * head_dim) or v.shape != (T, n_kv_heads * hdv):
-        raise KernelError(f"cache_store_e4m3: keys {tuple(k.shape)} and values {tuple(v.shape)} do "
-                          f"not fit {n_kv_heads} heads of {head_dim} and {hdv}")
-    _require(k.dtype == v.dtype, f"cache_store_e4m3: keys {k.dtype} and values {v.dtype} differ")
+    dev = _raw_device() if _raw_device is not None else torch.cuda.current_device()
+    T, B = len(k), len(slots)
+    pages, page = len(kp), view.page
+    scales = (pages, n_kv_heads)
+    # (all at once: a call of one token is mostly its checks)
+    if not (dev == k.get_device() == v.get_device() == kp.get_device() == vp.get_device() ==
+            ks.get_device() == vs.get_device() == table.get_device() == cu.get_device() ==
+            slots.get_device() == lens.get_device() and
+            k.shape == (T, n_kv_heads * head_dim) and v.shape == (T, n_kv_heads * hdv) and
+            k.dtype is v.dtype and kp.dtype is E4M3 and vp.dtype is E4M3 and
+            ks.dtype is torch.float32 and vs.dtype is torch.float32 and
+            table.dtype is cu.dtype is slots.dtype is lens.dtype is torch.int32 and
+            kp.shape == (pages, page, n_kv_heads, head_dim) and
+            vp.shape == (pages, page, n_kv_heads, hdv) and ks.shape == scales and
+            vs.shape == scales and cu.shape == (B + 1,) and lens.shape == (B,) and
+            slots.shape == (B,) and table.dim() == 2 and
+            kp.is_contiguous() and vp.is_contiguous() and ks.is_contiguous() and
+            vs.is_contiguous() and table.is_contiguous() and cu.is_contiguous() and
+            slots.is_contiguous() and lens.is_contiguous()):
+        _refuse_store(k, v, view, ctx, n_kv_heads, head_dim, hdv)
     (ldk, one), (ldv, one_v) = k.stride(), v.stride()
-    _require(one == 1 and one_v == 1, "cache_store_e4m3: elements of a row must be adjacent")
-    n_slots, max_pages, n_pages = _e4m3_view(view, n_kv_heads, head_dim, hdv, "cache_store_e4m3")
-    _i32(cu, "cu_seqlens"); _i32(slots, "slots"); _i32(lens, "lens")
-    _require(cu.numel() == B + 1 and lens.numel() == B and cu.is_contiguous() and
-             slots.is_contiguous() and lens.is_contiguous(),
-             "cache_store_e4m3: cu_seqlens [B + 1], slots [B] and lens [B] do not fit")
+    if one != 1 or one_v != 1:
+        _refuse_store(k, v, view, ctx, n_kv_heads, head_dim, hdv)
+    n_slots, max_pages = table.shape
+    code = dtype_code(k.dtype)
     with _span("cache_store", T * n_kv_heads * (head_dim + hdv) * (k.element_size() + 1)) \
-            if _watched() else _UNWATCHED:
-        _check(library().agv_cache_store_e4m3(
-            k.data_ptr(), ldk, v.data_ptr(), ldv, dtype_code(k.dtype), cu.data_ptr(),
-            slots.data_ptr(), lens.data_ptr(), B, T, int(ctx.max_new), n_kv_heads, head_dim, hdv,
-            kp.data_ptr(), vp.data_ptr(), ks.data_ptr(), vs.data_ptr(), table.data_ptr(), n_slots,
-            max_pages, view.page, view.cap, n_pages, _stream_handle()))
+            if _perf is not None or NVTX else _UNWATCHED:
+        rc = (_lib or library()).agv_cache_store_e4m3(
+            k.data_ptr(), ldk, v.data_ptr(), ldv, code, cu.data_ptr(), slots.data_ptr(),
+            lens.data_ptr(), B, T, int(ctx.max_new), n_kv_heads, head_dim, hdv, kp.data_ptr(),
+            vp.data_ptr(), ks.data_ptr(), vs.data_ptr(), table.data_ptr(), n_slots, max_pages, page,
+            view.cap, pages, _stream_handle())
+    if rc:
+        _check(rc)
 
 
 def attention_decode_e4m3(q: torch.Tensor, out: torch.Tensor, view, ctx, n_heads: int,
@@ -2132,49 +2170,61 @@ def attention_decode_e4m3(q: torch.Tensor, out: torch.Tensor, view, ctx, n_heads
     whole)."""
     hdv = value_dim or head_dim
     slots, positions = ctx.slots, ctx.positions
-    _require(e4m3_head_supported(head_dim, hdv),
-             f"attention_decode_e4m3: head sizes {head_dim} and {hdv} must be multiples of 16 up to "
-             f"{E4M3_MAX_HEAD}")
     kp, vp, ks, vs, table = view.k_pool, view.v_pool, view.k_scale, view.v_scale, view.page_table
-    _on_current_device(q, out, kp, vp, ks, vs, table, slots, positions, sinks, dist_bias)
-    B = q.shape[0]
-    if q.shape != (B, n_heads * head_dim) or q.stride(1) != 1:
-        raise KernelError(f"attention_decode_e4m3: queries {tuple(q.shape)} are not [B, {n_heads} * "
-                          f"{head_dim}]")
-    if out.dtype != q.dtype or out.shape != (B, n_heads * hdv) or not out.is_contiguous():
-        raise KernelError(f"attention_decode_e4m3: the output must be contiguous [{B}, "
-                          f"{n_heads * hdv}] of {q.dtype}")
-    n_slots, max_pages, n_pages = _e4m3_view(view, n_kv_heads, head_dim, hdv, "attention_decode_e4m3")
-    _i32(slots, "slots"); _i32(positions, "positions")
-    _require(slots.numel() == B and positions.numel() == B and slots.is_contiguous() and
-             positions.is_contiguous(), "attention_decode_e4m3: one slot and position per query")
+    if head_dim % 16 or hdv % 16 or not (0 < head_dim <= E4M3_MAX_HEAD and 0 < hdv <= E4M3_MAX_HEAD):
+        raise KernelError(f"attention_decode_e4m3: head sizes {head_dim} and {hdv} must be multiples "
+                          f"of 16 up to {E4M3_MAX_HEAD}")
+    dev = _raw_device() if _raw_device is not None else torch.cuda.current_device()
+    B, pages, page = len(q), len(kp), view.page
+    scales = (pages, n_kv_heads)
+    dtype = q.dtype
+    if not (dev == q.get_device() == out.get_device() == kp.get_device() == vp.get_device() ==
+            ks.get_device() == vs.get_device() == table.get_device() == slots.get_device() ==
+            positions.get_device() and
+            q.shape == (B, n_heads * head_dim) and out.shape == (B, n_heads * hdv) and
+            out.dtype is dtype and kp.dtype is E4M3 and vp.dtype is E4M3 and
+            ks.dtype is torch.float32 and vs.dtype is torch.float32 and
+            table.dtype is slots.dtype is positions.dtype is torch.int32 and
+            kp.shape == (pages, page, n_kv_heads, head_dim) and
+            vp.shape == (pages, page, n_kv_heads, hdv) and ks.shape == scales and
+            vs.shape == scales and slots.shape == (B,) and positions.shape == (B,) and
+            table.dim() == 2 and out.is_contiguous() and kp.is_contiguous() and
+            vp.is_contiguous() and ks.is_contiguous() and vs.is_contiguous() and
+            table.is_contiguous() and slots.is_contiguous() and positions.is_contiguous()):
+        _refuse_attend(q, out, view, ctx, n_heads, n_kv_heads, head_dim, hdv)
+    ldq, one = q.stride()
+    if one != 1:
+        _refuse_attend(q, out, view, ctx, n_heads, n_kv_heads, head_dim, hdv)
+    n_slots, max_pages = table.shape
+    sink_at = bias_at = None
+    n_dist = 0
     if sinks is not None:
-        _f32(sinks, "sinks")
+        _on_current_device(sinks); _f32(sinks, "sinks")
         _require(sinks.numel() == n_heads and sinks.is_contiguous(),
                  "attention_decode_e4m3: one sink per query head")
-    n_dist = 0
+        sink_at = sinks.data_ptr()
     if dist_bias is not None:
-        _f32(dist_bias, "dist_bias")
+        _on_current_device(dist_bias); _f32(dist_bias, "dist_bias")
         _require(dist_bias.dim() == 2 and dist_bias.shape[0] == n_heads and
                  dist_bias.is_contiguous(),
                  "attention_decode_e4m3: the bias by distance is [heads, distances]")
-        n_dist = dist_bias.shape[1]
+        bias_at, n_dist = dist_bias.data_ptr(), dist_bias.shape[1]
     max_keys = max(1, min(abs(window) + keep_first, ctx.max_len) if window else ctx.max_len)
-    lib = library()
+    lib = _lib or library()
     floats = lib.agv_attention_decode_e4m3_scratch(B, n_heads, n_kv_heads, head_dim, hdv, max_keys)
     if floats < 0:
         _check(floats)
     partial = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
     with _span(op, *_attention_cost(ctx, q, None, None, out, n_heads, head_dim, window, n_kv_heads,
-                                    1)) if _watched() else _UNWATCHED:
-        _check(lib.agv_attention_decode_e4m3(
-            q.data_ptr(), q.stride(0), out.data_ptr(), dtype_code(q.dtype), kp.data_ptr(),
-            vp.data_ptr(), ks.data_ptr(), vs.data_ptr(), table.data_ptr(), n_slots, max_pages,
-            view.page, view.cap, n_pages, slots.data_ptr(), positions.data_ptr(), B, n_heads,
-            n_kv_heads, head_dim, hdv, scale, window, keep_first,
-            sinks.data_ptr() if sinks is not None else None,
-            dist_bias.data_ptr() if dist_bias is not None else None, n_dist, softcap, max_keys,
-            partial.data_ptr() if partial is not None else None, floats, _stream_handle()))
+                                    1)) if _perf is not None or NVTX else _UNWATCHED:
+        rc = lib.agv_attention_decode_e4m3(
+            q.data_ptr(), ldq, out.data_ptr(), dtype_code(dtype), kp.data_ptr(), vp.data_ptr(),
+            ks.data_ptr(), vs.data_ptr(), table.data_ptr(), n_slots, max_pages, page, view.cap,
+            pages, slots.data_ptr(), positions.data_ptr(), B, n_heads, n_kv_heads, head_dim, hdv,
+            scale, window, keep_first, sink_at, bias_at, n_dist, softcap, max_keys,
+            partial.data_ptr() if floats else None, floats, _stream_handle())
+    if rc:
+        _check(rc)
 
 
 # ------------------------------------------------------------- log-probabilities
@@ -2184,7 +2234,8 @@ LOGPROBS_MAX_TOP = 32
 class TokenLogprobs:
     """What ``token_logprobs`` finds for R rows: ``logprob`` and ``entropy`` [R] (32-bit, nats),
     ``rank`` [R] (int32; 1 = the greatest logit), ``top_ids`` [R, top] (int32) and
-    ``top_logprobs`` [R, top] (32-bit), greatest first, equal ones by index."""
+    ``top_logprobs`` [R, top] (32-bit), greatest first, equal ones by index (both None for a
+    ``top`` of 0)."""
     __slots__ = ("logprob", "entropy", "rank", "top_ids", "top_logprobs")
 
 
@@ -2212,31 +2263,39 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
     ``packed`` (32-bit, ``token_logprobs_words`` values): everything goes there, one after the
     other, so that one copy brings it to the host (``unpack_token_logprobs``), and None is
     returned."""
-    _on_current_device(logits, tokens, packed)
-    _require(logits.dim() == 2 and logits.stride(1) == 1, "token_logprobs: logits must be [rows, vocabulary]")
-    R, V = logits.shape
-    _i32(tokens, "tokens")
-    _require(tokens.numel() == R and tokens.is_contiguous(), f"token_logprobs: one token for each of {R} rows")
+    dev = _raw_device() if _raw_device is not None else torch.cuda.current_device()
+    if not (dev == logits.get_device() == tokens.get_device()):
+        _on_current_device(logits, tokens)
+    shape = logits.shape
+    _require(len(shape) == 2 and logits.stride(1) == 1, "token_logprobs: logits must be [rows, vocabulary]")
+    R, V = shape
+    if tokens.dtype is not torch.int32:
+        _i32(tokens, "tokens")
+    _require(tokens.numel() == R and tokens.is_contiguous(), "token_logprobs: one token for each row")
     if not (0 <= top <= V and top <= LOGPROBS_MAX_TOP):
         raise KernelError(f"token_logprobs: top {top} must lie in 0..{min(V, LOGPROBS_MAX_TOP)}")
     r = None
     if packed is None:
-        r, new, i32, dev = TokenLogprobs(), torch.empty, torch.int32, logits.device
-        r.logprob = new(R, dtype=torch.float32, device=dev)
-        r.entropy = new(R, dtype=torch.float32, device=dev)
-        r.rank = new(R, dtype=i32, device=dev)
-        r.top_ids = new((R, top), dtype=i32, device=dev)
-        r.top_logprobs = new((R, top), dtype=torch.float32, device=dev)
-        out = (r.logprob.data_ptr(), r.entropy.data_ptr(), r.rank.data_ptr(), r.top_ids.data_ptr(),
-               r.top_logprobs.data_ptr())
+        r, new, f32, i32, on = TokenLogprobs(), torch.empty, torch.float32, torch.int32, logits.device
+        r.logprob = a = new(R, dtype=f32, device=on)
+        r.entropy = b = new(R, dtype=f32, device=on)
+        r.rank = c = new(R, dtype=i32, device=on)
+        r.top_ids = r.top_logprobs = None
+        out = (a.data_ptr(), b.data_ptr(), c.data_ptr(), None, None)
+        if top:
+            r.top_ids = a = new((R, top), dtype=i32, device=on)
+            r.top_logprobs = b = new((R, top), dtype=f32, device=on)
+            out = out[:3] + (a.data_ptr(), b.data_ptr())
     else:
-        _f32(packed, "packed")
+        _on_current_device(packed); _f32(packed, "packed")
         _require(packed.is_contiguous() and packed.numel() >= token_logprobs_words(R, top),
                  f"token_logprobs: packed must hold {token_logprobs_words(R, top)} values")
         at, n = packed.data_ptr(), 4 * R
         out = (at, at + n, at + 2 * n, at + 3 * n, at + (3 + top) * n)
-    with _span("token_logprobs", _nbytes(logits)) if _watched() else _UNWATCHED:
-        _check(library().agv_token_logprobs(
+    with _span("token_logprobs", _nbytes(logits)) if _perf is not None or NVTX else _UNWATCHED:
+        rc = (_lib or library()).agv_token_logprobs(
             logits.data_ptr(), logits.stride(0), dtype_code(logits.dtype), R, V, tokens.data_ptr(),
-            top, *out, _stream_handle()))
+            top, *out, _stream_handle())
+    if rc:
+        _check(rc)
     return r

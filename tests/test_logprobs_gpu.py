@@ -22,6 +22,9 @@ def check(logits, tokens, top):
     lp, ent, rank, ids, tlp, spread = P.logprobs(logits, tokens, top)
     R, V = logits.shape
     assert torch.equal(r.rank.long(), rank)
+    if top == 0:
+        assert r.top_ids is None and r.top_logprobs is None
+        r.top_ids, r.top_logprobs = ids, tlp
     assert r.top_ids.shape == (R, top) and torch.equal(r.top_ids.long(), ids)
     a = (V / 256 + 64) * 2.0 ** -24 + 2.0 ** -21 + 2.0 ** -23 * spread
     none = torch.isnan(lp)
@@ -154,6 +157,9 @@ def test_packed_results():
         assert (packed[-5:] == 0).all()
         for a, b in zip(kernels.unpack_token_logprobs(packed.cpu().numpy(), R, top),
                         (r.logprob, r.entropy, r.rank, r.top_ids, r.top_logprobs)):
+            if b is None:
+                assert a.size == 0
+                continue
             assert a.shape == b.shape and (a == b.cpu().numpy()).all()
         with pytest.raises(kernels.KernelError, match="packed"):
             kernels.token_logprobs(x, t, top, packed=packed[:2])
