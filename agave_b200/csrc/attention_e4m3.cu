@@ -33,6 +33,7 @@ constexpr int AE_THREADS = 32 * AE_WARPS;
 constexpr int AE_TILE = 16 * AE_WARPS;        // positions that a CTA's warps take together
 constexpr int AE_HEADS = 8;                   // query heads of a row
 constexpr int AE_MAX_DIM = 256;
+constexpr float AE_LEAST_SCALE = 7.8886090522101181e-31f;     // 2^-100: what the values' scales are held against at least
 
 struct AttendE4 {
     const void* q;
@@ -257,7 +258,8 @@ __device__ __forceinline__ void share_row(const AttendE4& a, float* red, float (
 }
 
 // ---------------------------------------------------------------- the walk over the keys
-template <typename T, int DIM>
+// EXTRAS: a soft cap or a bias by distance.
+template <typename T, int DIM, bool EXTRAS>
 __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kernel(const AttendE4 a) {
     using S = Tile<DIM>;
     constexpr bool SPLIT = sizeof(T) == 4;                       // two halves for a 32-bit value
@@ -440,160 +442,158 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
             }
             // this thread's columns of the scores and sums: heads 2 c and 2 c + 1
             constexpr float LOG2E = 1.4426950408889634f;
-            const bool extras = a.softcap > 0.f || a.dist_bias;
-            const float unit = extras ? a.scale : a.scale * LOG2E;
+            const float unit = EXTRAS ? a.scale : a.scale * LOG2E;
             const float f0 = __shfl_sync(0xffffffffu, qf, 8 * c) * unit;
             const float f1 = __shfl_sync(0xffffffffu, qf, 8 * c + 4) * unit;
             const float* bias = a.dist_bias ? a.dist_bias + (size_t)min(h0 + 2 * c, a.nh - 1) * a.n_dist : nullptr;
             const float* bias1 = a.dist_bias ? a.dist_bias + (size_t)min(h0 + 2 * c + 1, a.nh - 1) * a.n_dist : nullptr;
 
-            float o[NT][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, vref = 0.f, vlast = -1.f, vf = 0.f;
+            float o[NT][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+            float vref = AE_LEAST_SCALE, to_half = 16384.f / AE_LEAST_SCALE;
 #pragma unroll
             for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
 
+            // K q^T of a stage: positions r, r + 8 of heads 2 c, 2 c + 1, without any factor
+            auto products = [&](int stage, float (&s)[4]) {
+                const unsigned char* K = mine + stage * S::STAGE + r * S::KS + c * 16;
+                const int half = DIM > 64 ? (r & 1) * 64 : 0;
+                float x[2][4] = {};
+                float y[2][4] = {};
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) {
+                    const unsigned char* at = K + q * 64 + (q & 1 ? -half : half);
+                    const uint4 ka = *reinterpret_cast<const uint4*>(at);
+                    const uint4 kb = *reinterpret_cast<const uint4*>(at + 8 * S::KS);
+                    const unsigned wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+#pragma unroll
+                    for (int f = 0; f < 4; ++f) {
+                        unsigned a0, a1, a2, a3;
+                        e4m3_word(wa[f], a0, a2);
+                        e4m3_word(wb[f], a1, a3);
+                        mma16816(x[f & 1], a0, a1, a2, a3, qh[q][2 * f], qh[q][2 * f + 1]);
+                        if (SPLIT) mma16816(y[f & 1], a0, a1, a2, a3, ql[q][2 * f], ql[q][2 * f + 1]);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[e] = x[0][e] + x[1][e] + (SPLIT ? y[0][e] + y[1][e] : 0.f);
+            };
+            copies_wait<S::STAGES - 2>();
+            __syncwarp();
+            float p[4];
+            products(0, p);
             int stage = 0;
-            for (; now.t < t_end; advance(now)) {
-                const int ahead = stage == 0 ? S::STAGES - 1 : stage - 1;
-                issue(next, next_page, ahead);
+            while (now.t < t_end) {
+                issue(next, next_page, stage == 0 ? S::STAGES - 1 : stage - 1);
                 advance(next);
                 next_page = page_of(next);
-                copies_wait<S::STAGES - 1>();
+                copies_wait<S::STAGES - 2>();                    // the tile after this one is there
                 __syncwarp();
+                // Its products are independent of what follows, this tile's softmax and sums, whose
+                // chains of instructions they fill (behind the last tile: of anything, and not used).
+                const int after = stage + 1 == S::STAGES ? 0 : stage + 1;
+                float p_after[4];
+                products(after, p_after);
+
                 const int j0 = now.j;
-                if (j0 <= s.p && meta[warp][stage][2] != 0.f) {
-                    const unsigned char* V = mine + stage * S::STAGE + 16 * S::KS;
-                    const unsigned char* K = mine + stage * S::STAGE + r * S::KS + c * 16;
-                    const int half = DIM > 64 ? (r & 1) * 64 : 0;
-                    const float ks = meta[warp][stage][0], vs = meta[warp][stage][1];
-                    float x[2][4] = {};
-                    float y[2][4] = {};
+                const unsigned char* V = mine + stage * S::STAGE + 16 * S::KS;
+                const bool there = meta[warp][stage][2] != 0.f;
+                const float ks = meta[warp][stage][0], vs = there ? meta[warp][stage][1] : 0.f;
+                const float g0 = ks * f0, g1 = ks * f1;
+                // scores of positions j0 + r, j0 + r + 8 in units of ln 2
+                const int ja = j0 + r, jb = ja + 8;
+                const bool see_a = there && ja <= s.p && (ja >= s.first || ja < s.kept);
+                const bool see_b = there && jb <= s.p && (jb >= s.first || jb < s.kept);
 #pragma unroll
-                    for (int q = 0; q < NQ; ++q) {
-                        const unsigned char* at = K + q * 64 + (q & 1 ? -half : half);
-                        const uint4 ka = *reinterpret_cast<const uint4*>(at);
-                        const uint4 kb = *reinterpret_cast<const uint4*>(at + 8 * S::KS);
-                        const unsigned wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
-#pragma unroll
-                        for (int f = 0; f < 4; ++f) {
-                            unsigned a0, a1, a2, a3;
-                            e4m3_word(wa[f], a0, a2);
-                            e4m3_word(wb[f], a1, a3);
-                            mma16816(x[f & 1], a0, a1, a2, a3, qh[q][2 * f], qh[q][2 * f + 1]);
-                            if (SPLIT) mma16816(y[f & 1], a0, a1, a2, a3, ql[q][2 * f], ql[q][2 * f + 1]);
-                        }
+                for (int e = 0; e < 4; ++e) {
+                    p[e] *= e & 1 ? g1 : g0;
+                    if (EXTRAS) {
+                        if (a.softcap > 0.f) p[e] = soft_capped(p[e], a.softcap);
+                        if (a.dist_bias) p[e] += (e & 1 ? bias1 : bias)[min(max(s.p - (e >> 1 ? jb : ja), 0), a.n_dist - 1)];
+                        p[e] *= LOG2E;
                     }
-                    // scores of positions j0 + r, j0 + r + 8 in units of ln 2
-                    float p[4];
-                    const float g0 = ks * f0, g1 = ks * f1;
+                    if (!(e >> 1 ? see_b : see_a)) p[e] = -INFINITY;
+                }
+                float t0 = fmaxf(p[0], p[2]), t1 = fmaxf(p[1], p[3]);
+#pragma unroll
+                for (int w = 4; w < 32; w <<= 1) {
+                    t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, w));
+                    t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, w));
+                }
+                t0 = fmaxf(t0, m0);
+                t1 = fmaxf(t1, m1);
+                const float u0 = t0 == -INFINITY ? 0.f : t0, u1 = t1 == -INFINITY ? 0.f : t1;
+                float k0 = ex2(m0 - u0), k1 = ex2(m1 - u1);
+                m0 = t0;
+                m1 = t1;
+                p[0] = ex2(p[0] - u0);
+                p[1] = ex2(p[1] - u1);
+                p[2] = ex2(p[2] - u0);
+                p[3] = ex2(p[3] - u1);
+                l0 = fmaf(l0, k0, p[0] + p[2]);
+                l1 = fmaf(l1, k1, p[1] + p[3]);
+                // a greater maximum, or a greater scale of values than any before
+                if (__any_sync(0xffffffffu, k0 != 1.f || k1 != 1.f || vs > vref)) {
+                    if (vs > vref) {
+                        k0 *= vref / vs;
+                        k1 *= vref / vs;
+                        vref = vs;
+                        to_half = 16384.f / vref;
+                    }
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        o[t][0] *= k0;
+                        o[t][1] *= k1;
+                        o[t][2] *= k0;
+                        o[t][3] *= k1;
+                    }
+                }
+                const float vf = vs * to_half;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[e] *= vf;
+                const unsigned h0w = half2_of(p[0], p[1]), h1w = half2_of(p[2], p[3]);
+                const unsigned b0 = transposed(h0w), b1 = transposed(h1w);
+                unsigned c0 = 0, c1 = 0;
+                if (SPLIT) {
+                    const float2 w0 = float2_of(h0w), w1 = float2_of(h1w);
+                    c0 = transposed(half2_of(p[0] - w0.x, p[1] - w0.y));
+                    c1 = transposed(half2_of(p[2] - w1.x, p[3] - w1.y));
+                }
+                // values: dimensions q * 8 VB + r * VB .. of positions 2 c, 2 c + 1, 2 c + 8, 2 c + 9
+#pragma unroll
+                for (int q = 0; q < NV; ++q) {
+                    unsigned w[4][VB / 4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        p[e] = x[0][e] + x[1][e];
-                        if (SPLIT) p[e] += y[0][e] + y[1][e];
-                        p[e] *= e & 1 ? g1 : g0;
-                    }
-                    if (extras) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int j = j0 + r + (e >> 1) * 8;
-                            if (a.softcap > 0.f) p[e] = soft_capped(p[e], a.softcap);
-                            if (a.dist_bias) p[e] += (e & 1 ? bias1 : bias)[min(max(s.p - j, 0), a.n_dist - 1)];
-                            p[e] *= LOG2E;
+                        const unsigned char* at = V + (2 * c + (e & 1) + (e >> 1) * 8) * S::VS + q * 8 * VB + r * VB;
+                        if constexpr (VB == 16) {
+                            const uint4 u = *reinterpret_cast<const uint4*>(at);
+                            w[e][0] = u.x; w[e][1] = u.y; w[e][2] = u.z; w[e][3] = u.w;
+                        } else {
+                            const uint2 u = *reinterpret_cast<const uint2*>(at);
+                            w[e][0] = u.x; w[e][1] = u.y;
                         }
                     }
-                    if (j0 < s.first || j0 + 15 > s.p) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int j = j0 + r + (e >> 1) * 8;
-                            if (j > s.p || (j < s.first && j >= s.kept)) p[e] = -INFINITY;
-                        }
-                    }
-                    float t0 = fmaxf(p[0], p[2]), t1 = fmaxf(p[1], p[3]);
-#pragma unroll
-                    for (int w = 4; w < 32; w <<= 1) {
-                        t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, w));
-                        t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, w));
-                    }
-                    t0 = fmaxf(t0, m0);
-                    t1 = fmaxf(t1, m1);
-                    const float u0 = t0 == -INFINITY ? 0.f : t0, u1 = t1 == -INFINITY ? 0.f : t1;
-                    float k0 = ex2(m0 - u0), k1 = ex2(m1 - u1);
-                    m0 = t0;
-                    m1 = t1;
-                    l0 *= k0;
-                    l1 *= k1;
-                    if (vs != vlast) {
-                        vlast = vs;
-                        if (!(vs <= vref)) {                      // the greatest scale so far
-                            k0 *= vref / vs;
-                            k1 *= vref / vs;
-                            vref = vs;
-                        }
-                        vf = vs / vref * 16384.f;
-                    }
-                    if (__any_sync(0xffffffffu, k0 != 1.f || k1 != 1.f)) {
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            o[t][0] *= k0;
-                            o[t][1] *= k1;
-                            o[t][2] *= k0;
-                            o[t][3] *= k1;
-                        }
-                    }
-                    p[0] = ex2(p[0] - u0);
-                    p[1] = ex2(p[1] - u1);
-                    p[2] = ex2(p[2] - u0);
-                    p[3] = ex2(p[3] - u1);
-                    l0 += p[0] + p[2];
-                    l1 += p[1] + p[3];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) p[e] *= vf;
-                    const unsigned h0w = half2_of(p[0], p[1]), h1w = half2_of(p[2], p[3]);
-                    const unsigned b0 = transposed(h0w), b1 = transposed(h1w);
-                    unsigned c0 = 0, c1 = 0;
-                    if (SPLIT) {
-                        const float2 w0 = float2_of(h0w), w1 = float2_of(h1w);
-                        c0 = transposed(half2_of(p[0] - w0.x, p[1] - w0.y));
-                        c1 = transposed(half2_of(p[2] - w1.x, p[3] - w1.y));
-                    }
-                    // values: dimensions q * 8 VB + r * VB .. of positions 2 c, 2 c + 1, 2 c + 8, 2 c + 9
-#pragma unroll
-                    for (int q = 0; q < NV; ++q) {
-                        unsigned w[4][VB / 4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const unsigned char* at = V + (2 * c + (e & 1) + (e >> 1) * 8) * S::VS + q * 8 * VB + r * VB;
-                            if constexpr (VB == 16) {
-                                const uint4 u = *reinterpret_cast<const uint4*>(at);
-                                w[e][0] = u.x; w[e][1] = u.y; w[e][2] = u.z; w[e][3] = u.w;
-                            } else {
-                                const uint2 u = *reinterpret_cast<const uint2*>(at);
-                                w[e][0] = u.x; w[e][1] = u.y;
-                            }
-                        }
-#pragma unroll
-                        for (int f = 0; f < VB / 4; ++f) {
-                            const unsigned la = __byte_perm(w[0][f], w[1][f], 0x5140), lb = __byte_perm(w[0][f], w[1][f], 0x7362);
-                            const unsigned ha = __byte_perm(w[2][f], w[3][f], 0x5140), hb = __byte_perm(w[2][f], w[3][f], 0x7362);
-                            const int t = q * (VB / 2) + 2 * f;
-                            {
-                                unsigned a0, a1, a2, a3;
-                                e4m3_word(la, a0, a1);
-                                e4m3_word(ha, a2, a3);
-                                mma16816(o[t], a0, a1, a2, a3, b0, b1);
-                                if (SPLIT) mma16816(o[t], a0, a1, a2, a3, c0, c1);
-                            }
-                            {
-                                unsigned a0, a1, a2, a3;
-                                e4m3_word(lb, a0, a1);
-                                e4m3_word(hb, a2, a3);
-                                mma16816(o[t + 1], a0, a1, a2, a3, b0, b1);
-                                if (SPLIT) mma16816(o[t + 1], a0, a1, a2, a3, c0, c1);
-                            }
-                        }
+                    for (int f = 0; f < VB / 4; ++f) {
+                        const unsigned la = __byte_perm(w[0][f], w[1][f], 0x5140), lb = __byte_perm(w[0][f], w[1][f], 0x7362);
+                        const unsigned ha = __byte_perm(w[2][f], w[3][f], 0x5140), hb = __byte_perm(w[2][f], w[3][f], 0x7362);
+                        const int t = q * (VB / 2) + 2 * f;
+                        unsigned a0, a1, a2, a3;
+                        e4m3_word(la, a0, a1);
+                        e4m3_word(ha, a2, a3);
+                        mma16816(o[t], a0, a1, a2, a3, b0, b1);
+                        if (SPLIT) mma16816(o[t], a0, a1, a2, a3, c0, c1);
+                        e4m3_word(lb, a0, a1);
+                        e4m3_word(hb, a2, a3);
+                        mma16816(o[t + 1], a0, a1, a2, a3, b0, b1);
+                        if (SPLIT) mma16816(o[t + 1], a0, a1, a2, a3, c0, c1);
                     }
                 }
                 __syncwarp();                                    // the stage may be written again
-                stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+                stage = after;
+                advance(now);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[e] = p_after[e];
             }
             // ---- the warps' results together
             copies_wait<0>();
@@ -791,19 +791,18 @@ Plan plan_of(int B, int nh, int nkv, int hd, int hdv, int max_keys) {
     if (p.split && p.ctas > AE_MAX_CTAS) p.ctas = AE_MAX_CTAS;
     return p;
 }
-template <typename T, int DIM>
+template <typename T, int DIM, bool EXTRAS>
 int launch(const AttendE4& a, const Plan& p, cudaStream_t stream) {
     static std::atomic<unsigned long long> ready{0};             // devices on which the kernel has been set up
+    const auto kern = attend_e4m3_kernel<T, DIM, EXTRAS>;
     int dev = 0;
     AGV_CUDA_OK(cudaGetDevice(&dev));
     if (!(ready.load() >> (dev & 63) & 1)) {
-        AGV_CUDA_OK(cudaFuncSetAttribute(attend_e4m3_kernel<T, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         Tile<DIM>::SMEM));
-        AGV_CUDA_OK(cudaFuncSetAttribute(attend_e4m3_kernel<T, DIM>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        AGV_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<DIM>::SMEM));
+        AGV_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         ready.fetch_or(1ull << (dev & 63));
     }
-    agv_launch_cluster(attend_e4m3_kernel<T, DIM>, p.ctas, AE_THREADS, Tile<DIM>::SMEM, stream,
-                       dim3(p.split ? 1 : p.cluster), a);
+    agv_launch_cluster(kern, p.ctas, AE_THREADS, Tile<DIM>::SMEM, stream, dim3(p.split ? 1 : p.cluster), a);
     AGV_LAUNCH_OK("attend_e4m3_kernel");
     if (p.split && p.ctas > 1) {
         const int heads = a.nh / a.nkv < AE_HEADS ? a.nh / a.nkv : AE_HEADS;
@@ -812,11 +811,16 @@ int launch(const AttendE4& a, const Plan& p, cudaStream_t stream) {
     }
     return 0;
 }
+template <typename T, int DIM>
+int launch_extras(const AttendE4& a, const Plan& p, cudaStream_t stream) {
+    if (a.softcap > 0.f || a.dist_bias) return launch<T, DIM, true>(a, p, stream);
+    return launch<T, DIM, false>(a, p, stream);
+}
 template <typename T>
 int launch_dim(const AttendE4& a, const Plan& p, cudaStream_t stream) {
-    if (p.dim == 64) return launch<T, 64>(a, p, stream);
-    if (p.dim == 128) return launch<T, 128>(a, p, stream);
-    return launch<T, 256>(a, p, stream);
+    if (p.dim == 64) return launch_extras<T, 64>(a, p, stream);
+    if (p.dim == 128) return launch_extras<T, 128>(a, p, stream);
+    return launch_extras<T, 256>(a, p, stream);
 }
 
 }  // namespace
