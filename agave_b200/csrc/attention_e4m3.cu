@@ -4,11 +4,14 @@
 // s_aj = cap(scale * q_a . k_j) + bias; one pass over the keys with a running maximum m.
 //
 // What bounds it is reading each key and value once, hd + hdv bytes a position and kv head.  The
-// work, (sequence, kv head, up to 8 of its query heads) x pages of 64 positions, lies on one
-// line and every CTA takes an equal stretch of it whatever the sequences' lengths are; a CTA
-// whose stretch begins or ends inside a row leaves a partial result (sum, maximum, normaliser),
-// and a second kernel joins those.  The stretches follow from the positions on the device, so a
-// recorded launch serves every length.
+// pages of all sequences, 64 positions each, lie on one line, which is cut into equal stretches
+// whatever the sequences' lengths are; a CTA takes a stretch for one kv head and up to 8 of its query heads,
+// and where that begins or ends inside a sequence it leaves a partial result (sum, maximum,
+// normaliser), which a second kernel joins.  The stretches follow from the positions on the device,
+// so a recorded launch serves every length.  The CTAs of a stretch, a head each, lie beside each
+// other on the grid and go through it together: a head's 64 to 256 bytes of a position are a part
+// of what DRAM opens for it, and together they are all of it (64 sequences up to 8192 with 16
+// kv heads of 128: 238 us with stretches that lay along the heads, HEADTIME like this).
 //
 // In a CTA each of four warps takes 16 of a page's positions and runs for itself: its copies
 // (16-byte cp.async, ring of AE_STAGES tiles), its running maximum, its sums; the warps meet only at
@@ -185,8 +188,8 @@ __device__ __forceinline__ void find_tile(const AttendE4& a, int y, int* scan, f
     seq = scan[0];
     before = scan[1];
 }
-__device__ __forceinline__ long long stretch_start(long long units, int cta, int ctas) {
-    return units * cta / ctas;
+__device__ __forceinline__ int stretch_start(int total, int part, int stretches) {
+    return (int)((long long)total * part / stretches);
 }
 
 __device__ __forceinline__ void cluster_meet() {
@@ -277,21 +280,17 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
     unsigned char* mine = smem + warp * S::STAGES * S::STAGE;
     const unsigned mine_at = (unsigned)__cvta_generic_to_shared(mine);
 
-    // this CTA's stretch
-    int b, before, row;
-    long long left;                                              // units still to do
-    int tile;
+    // this CTA's row (a kv head and up to 8 of its query heads), sequence, tile and tiles left to do
+    int b, row, tile, left;
     if (a.partial) {
-        const int total = all_tiles<AE_THREADS>(a, scan, scratch);
-        const long long units = (long long)total * R;
-        const long long x0 = stretch_start(units, blockIdx.x, gridDim.x);
-        left = stretch_start(units, blockIdx.x + 1, gridDim.x) - x0;
+        const int total = all_tiles<AE_THREADS>(a, scan, scratch), stretches = gridDim.x / R, part = blockIdx.x / R;
+        const int x0 = stretch_start(total, part, stretches);
+        row = blockIdx.x % R;
+        left = stretch_start(total, part + 1, stretches) - x0;
         if (left == 0) return;
-        find_tile<AE_THREADS>(a, (int)(x0 / R), scan, scratch, b, before);
-        const int n = seen_by(a, b).tiles;
-        const long long in = x0 - (long long)before * R;
-        row = (int)(in / n);
-        tile = (int)(in - (long long)row * n);
+        int before;
+        find_tile<AE_THREADS>(a, x0, scan, scratch, b, before);
+        tile = x0 - before;
     } else {
         const int unit = blockIdx.x / a.cluster, part = blockIdx.x % a.cluster;
         b = unit / R;
@@ -306,7 +305,7 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
         const Seen s = seen_by(a, b);
         const int g = row / a.row_blocks, h0 = g * group + row % a.row_blocks * AE_HEADS;
         const int heads = min(AE_HEADS, (g + 1) * group - h0);
-        const int n = (int)min((long long)(s.tiles - tile), left);   // tiles of this segment
+        const int n = min(s.tiles - tile, left);                     // tiles of this segment
         const bool whole = n == s.tiles;
         if (s.slot < 0) {
             if (!shared_row || left > 0) {
@@ -668,54 +667,46 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
             }
             __syncthreads();
         }
-        // the next segment: the next row from its first tile on
+        // the next segment: the next sequence from its first tile on
         left -= n;
         ++segment;
         tile = 0;
-        if (++row == R) {
-            row = 0;
-            ++b;
-        }
+        ++b;
     }
 }
 
 // ---------------------------------------------------------------- rows of several CTAs
-// CTA (i, h) joins, for head h of 8, the row inside which the stretch of CTA i + 1 begins, if it is
-// the first to begin there.  First the partial results' weights, a thread each, then the sums:
+// CTA (i, h, r) joins, for head h of 8 of row r, the sequence inside which stretch i + 1 begins, if it
+// is the first to begin there.  First the partial results' weights, a thread each, then the sums:
 // DIM / 4 threads take a partial result, the CTA 8 to 32 of them at a time.
 constexpr int AE_JOIN_THREADS = 512;
-constexpr int AE_MAX_CTAS = 1024;
+constexpr int AE_MAX_STRETCHES = 1024;
 template <typename T, int DIM>
-__global__ void __launch_bounds__(AE_JOIN_THREADS) join_e4m3_kernel(const AttendE4 a, int ctas) {
+__global__ void __launch_bounds__(AE_JOIN_THREADS) join_e4m3_kernel(const AttendE4 a, int stretches) {
     using S = Tile<DIM>;
     __shared__ int scan[2];
-    __shared__ float weight[AE_MAX_CTAS];
-    __shared__ int slot[AE_MAX_CTAS];
+    __shared__ float weight[AE_MAX_STRETCHES];
+    __shared__ int slot[AE_MAX_STRETCHES];
     __shared__ float scratch[32];
     __shared__ float4 sums[AE_JOIN_THREADS];
     pdl_wait();
     pdl_launch_next();
-    const int R = a.nkv * a.row_blocks, group = a.nh / a.nkv, head = blockIdx.y, tid = threadIdx.x;
-    const int total = all_tiles<AE_JOIN_THREADS>(a, scan, scratch);
-    const long long units = (long long)total * R;
-    const int i = blockIdx.x + 1;
-    const long long x = stretch_start(units, i, ctas);
-    if (x >= units) return;
-    int b, before;
-    find_tile<AE_JOIN_THREADS>(a, (int)(x / R), scan, scratch, b, before);
-    const int n = seen_by(a, b).tiles;
-    const int row = (int)((x - (long long)before * R) / n);
-    const long long begin = (long long)before * R + (long long)row * n, end = begin + n;
-    if (x == begin || stretch_start(units, i - 1, ctas) > begin) return;      // not inside, not the first
+    const int R = a.nkv * a.row_blocks, group = a.nh / a.nkv, head = blockIdx.y, row = blockIdx.z, tid = threadIdx.x;
     const int g = row / a.row_blocks, h0 = g * group + row % a.row_blocks * AE_HEADS;
     if (h0 + head >= (g + 1) * group) return;
-    // the CTAs i - 1 .. last have a part of the row (but for those whose stretch is empty)
-    const int last = (int)((end * ctas - 1) / units), parts = last - i + 2;
+    const int total = all_tiles<AE_JOIN_THREADS>(a, scan, scratch);
+    const int i = blockIdx.x + 1, x = stretch_start(total, i, stretches);
+    if (x >= total) return;
+    int b, begin;
+    find_tile<AE_JOIN_THREADS>(a, x, scan, scratch, b, begin);
+    const int end = begin + seen_by(a, b).tiles;
+    if (x == begin || stretch_start(total, i - 1, stretches) > begin) return;  // not inside, not the first
+    // the stretches i - 1 .. last have a part of the sequence (but for empty ones)
+    const int last = (int)(((long long)end * stretches - 1) / total), parts = last - i + 2;
     float M = -INFINITY;
     for (int j = tid; j < parts; j += AE_JOIN_THREADS) {
-        const int cta = i - 1 + j;
-        const long long from = stretch_start(units, cta, ctas);
-        const int at = from == stretch_start(units, cta + 1, ctas) ? -1 : 2 * cta + (from < begin);
+        const int part = i - 1 + j, from = stretch_start(total, part, stretches);
+        const int at = from == stretch_start(total, part + 1, stretches) ? -1 : 2 * (part * R + row) + (from < begin);
         slot[j] = at;
         weight[j] = at < 0 ? -INFINITY : a.partial[(size_t)at * S::PART + AE_HEADS * DIM + 2 * head];
         M = fmaxf(M, weight[j]);
@@ -762,6 +753,7 @@ __global__ void __launch_bounds__(AE_JOIN_THREADS) join_e4m3_kernel(const Attend
 struct Plan {
     int dim, ctas;             // padded head size; CTAs of the launch
     bool split;                // stretches of an equal number of tiles, joined afterwards
+    int stretches;             // so many for each row
     int cluster;               // else: CTAs that share a row
 };
 int sm_count() {
@@ -786,9 +778,12 @@ Plan plan_of(int B, int nh, int nkv, int hd, int hdv, int max_keys) {
     p.cluster = 1;
     while (p.cluster < 16 && p.cluster < tiles && rows * p.cluster * 2 <= resident) p.cluster *= 2;
     p.split = tiles > 8 * p.cluster;
-    if (!p.split) p.ctas = (int)(rows * p.cluster);
-    else p.ctas = (int)(rows * tiles < resident ? rows * tiles : resident);
-    if (p.split && p.ctas > AE_MAX_CTAS) p.ctas = AE_MAX_CTAS;
+    const int R = (int)(rows / B);
+    long long stretches = resident / R;                          // all CTAs at a time
+    if (stretches > B * tiles) stretches = B * tiles;
+    if (stretches > AE_MAX_STRETCHES) stretches = AE_MAX_STRETCHES;
+    p.stretches = !p.split ? 0 : stretches < 1 ? 1 : (int)stretches;
+    p.ctas = p.split ? p.stretches * R : (int)(rows * p.cluster);
     return p;
 }
 template <typename T, int DIM, bool EXTRAS>
@@ -804,9 +799,10 @@ int launch(const AttendE4& a, const Plan& p, cudaStream_t stream) {
     }
     agv_launch_cluster(kern, p.ctas, AE_THREADS, Tile<DIM>::SMEM, stream, dim3(p.split ? 1 : p.cluster), a);
     AGV_LAUNCH_OK("attend_e4m3_kernel");
-    if (p.split && p.ctas > 1) {
+    if (p.stretches > 1) {
         const int heads = a.nh / a.nkv < AE_HEADS ? a.nh / a.nkv : AE_HEADS;
-        agv_launch(join_e4m3_kernel<T, DIM>, dim3(p.ctas - 1, heads), AE_JOIN_THREADS, 0, stream, a, p.ctas);
+        agv_launch(join_e4m3_kernel<T, DIM>, dim3(p.stretches - 1, heads, a.nkv * a.row_blocks), AE_JOIN_THREADS, 0, stream,
+                   a, p.stretches);
         AGV_LAUNCH_OK("join_e4m3_kernel");
     }
     return 0;
