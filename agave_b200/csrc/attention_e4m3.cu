@@ -11,7 +11,7 @@
 // so a recorded launch serves every length.  The CTAs of a stretch, a head each, lie beside each
 // other on the grid and go through it together: a head's 64 to 256 bytes of a position are a part
 // of what DRAM opens for it, and together they are all of it (64 sequences up to 8192 with 16
-// kv heads of 128: 238 us with stretches that lay along the heads, HEADTIME like this).
+// kv heads of 128: 238 us with stretches that lay along the heads, 191 like this).
 //
 // In a CTA each of four warps takes 16 of a page's positions and runs for itself: its copies
 // (16-byte cp.async, ring of AE_STAGES tiles), its running maximum, its sums; the warps meet only at
@@ -141,55 +141,72 @@ __device__ __forceinline__ Seen seen_by(const AttendE4& a, int b) {
     return s;
 }
 
-// The sequences' tiles on one line.  ``scan``: 2 ints of shared memory, ``scratch``: 32 floats of it.
-// All THREADS of a CTA take part and get the result.
-template <int THREADS>
-__device__ __forceinline__ int all_tiles(const AttendE4& a, int* scan, float* scratch) {
-    int n = 0;
-    for (int b = threadIdx.x; b < a.B; b += THREADS) n += seen_by(a, b).tiles;
-    n = __reduce_add_sync(0xffffffffu, n);
-    int* sums = reinterpret_cast<int*>(scratch);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = n;
-    __syncthreads();
-    return __reduce_add_sync(0xffffffffu, (threadIdx.x & 31) < THREADS / 32 ? sums[threadIdx.x & 31] : 0);
+__device__ __forceinline__ int stretch_start(int total, int part, int stretches) {
+    return (int)((long long)total * part / stretches);
 }
-// The sequence that tile y of the line belongs to, and the tiles before it.
-template <int THREADS>
-__device__ __forceinline__ void find_tile(const AttendE4& a, int y, int* scan, float* scratch, int& seq, int& before) {
+// Where a stretch begins: the tiles of all sequences, the stretch's first one and its end, the sequence
+// it lies in and the tiles before that sequence.
+struct Start {
+    int total, x0, x1, seq, before, tiles;
+};
+// The sequences' tiles on one line, and on it the stretch ``part`` of so many.  All AE_THREADS of
+// the CTA take part and get the result (seq -1 where it begins behind the last tile).
+__device__ __forceinline__ Start find_stretch(const AttendE4& a, int part, int stretches) {
+    __shared__ int sums[AE_WARPS], found[3];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int* sums = reinterpret_cast<int*>(scratch);
+    Start at;
+    // up to AE_THREADS sequences in one go, else all of them first and then one group after the other
+    int n = 0, b = threadIdx.x;
+    if (a.B <= AE_THREADS) {
+        n = b < a.B ? seen_by(a, b).tiles : 0;
+    } else {
+        int all = 0;
+        for (; b < a.B; b += AE_THREADS) all += seen_by(a, b).tiles;
+        all = __reduce_add_sync(0xffffffffu, all);
+        if (lane == 0) sums[warp] = all;
+        __syncthreads();
+        at.total = 0;
+#pragma unroll
+        for (int w = 0; w < AE_WARPS; ++w) at.total += sums[w];
+        __syncthreads();
+    }
+    at.seq = -1;
     int done = 0;
-    for (int base = 0; base < a.B; base += THREADS) {
-        const int b = base + threadIdx.x;
-        const int n = b < a.B ? seen_by(a, b).tiles : 0;
+    for (int base = 0; base < a.B; base += AE_THREADS) {
+        b = base + threadIdx.x;
+        if (a.B > AE_THREADS) n = b < a.B ? seen_by(a, b).tiles : 0;
         int upto = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int t = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= o) upto += t;
         }
-        __syncthreads();
         if (lane == 31) sums[warp] = upto;
         __syncthreads();
-        int total = 0;
+        int group = 0;
 #pragma unroll
-        for (int w = 0; w < THREADS / 32; ++w) {
+        for (int w = 0; w < AE_WARPS; ++w) {
             if (w < warp) upto += sums[w];
-            total += sums[w];
+            group += sums[w];
         }
-        if (y < done + total) {
-            if (y >= done + upto - n && y < done + upto) { scan[0] = b; scan[1] = done + upto - n; }
-            break;
+        if (a.B <= AE_THREADS) at.total = group;
+        at.x0 = stretch_start(at.total, part, stretches);
+        at.x1 = stretch_start(at.total, part + 1, stretches);
+        if (at.x0 >= at.total) return at;                        // (the same for every thread)
+        const bool here = at.x0 < done + group;
+        if (here && at.x0 >= done + upto - n && at.x0 < done + upto) {
+            found[0] = b;
+            found[1] = done + upto - n;
+            found[2] = n;
         }
-        done += total;
+        __syncthreads();
+        if (here) break;
+        done += group;
     }
-    __syncthreads();
-    seq = scan[0];
-    before = scan[1];
-}
-__device__ __forceinline__ int stretch_start(int total, int part, int stretches) {
-    return (int)((long long)total * part / stretches);
+    at.seq = found[0];
+    at.before = found[1];
+    at.tiles = found[2];
+    return at;
 }
 
 __device__ __forceinline__ void cluster_meet() {
@@ -269,8 +286,6 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
     constexpr int NQ = DIM / 64, NT = DIM / 16;
     constexpr int VB = DIM >= 128 ? 16 : 8, NV = DIM / (8 * VB); // bytes of values at a time, times
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ int scan[2];
-    __shared__ float scratch[32];
     __shared__ float stat[AE_WARPS][AE_HEADS][2];
     __shared__ float meta[AE_WARPS][S::STAGES][4];               // scales of keys and values, page is there
     pdl_wait();
@@ -283,14 +298,17 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
     // this CTA's row (a kv head and up to 8 of its query heads), sequence, tile and tiles left to do
     int b, row, tile, left;
     if (a.partial) {
-        const int total = all_tiles<AE_THREADS>(a, scan, scratch), stretches = gridDim.x / R, part = blockIdx.x / R;
-        const int x0 = stretch_start(total, part, stretches);
+        const int stretches = gridDim.x / R, part = blockIdx.x / R;
         row = blockIdx.x % R;
-        left = stretch_start(total, part + 1, stretches) - x0;
-        if (left == 0) return;
-        int before;
-        find_tile<AE_THREADS>(a, x0, scan, scratch, b, before);
-        tile = x0 - before;
+        const Start at = find_stretch(a, part, stretches);
+        // (what the join has to know of the stretch)
+        if (row == 0 && tid == 0)
+            reinterpret_cast<int4*>(a.partial)[part] =
+                make_int4(at.seq, at.before, at.seq < 0 ? 0 : at.before + at.tiles, at.total);
+        b = at.seq;
+        tile = at.x0 - at.before;
+        left = at.x1 - at.x0;
+        if (b < 0 || left == 0) return;
     } else {
         const int unit = blockIdx.x / a.cluster, part = blockIdx.x % a.cluster;
         b = unit / R;
@@ -632,7 +650,7 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
                 }
             }
             __syncthreads();
-            float* part = a.partial ? a.partial + (size_t)(2 * blockIdx.x + (segment > 0)) * S::PART : nullptr;
+            float* part = a.partial ? a.partial + gridDim.x / R * 4 + (size_t)(2 * blockIdx.x + (segment > 0)) * S::PART : nullptr;
             if (shared_row) {
                 share_row<T, DIM>(a, red, stat, b, h0, heads);
                 return;
@@ -676,7 +694,7 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
 }
 
 // ---------------------------------------------------------------- rows of several CTAs
-// CTA (i, h, r) joins, for head h of 8 of row r, the sequence inside which stretch i + 1 begins, if it
+// CTA (i, h, r) joins, for head h of 8 of row r (and every gridDim.y-th after it), the sequence inside which stretch i + 1 begins, if it
 // is the first to begin there.  First the partial results' weights, a thread each, then the sums:
 // DIM / 4 threads take a partial result, the CTA 8 to 32 of them at a time.
 constexpr int AE_JOIN_THREADS = 512;
@@ -684,69 +702,69 @@ constexpr int AE_MAX_STRETCHES = 1024;
 template <typename T, int DIM>
 __global__ void __launch_bounds__(AE_JOIN_THREADS) join_e4m3_kernel(const AttendE4 a, int stretches) {
     using S = Tile<DIM>;
-    __shared__ int scan[2];
     __shared__ float weight[AE_MAX_STRETCHES];
     __shared__ int slot[AE_MAX_STRETCHES];
     __shared__ float scratch[32];
     __shared__ float4 sums[AE_JOIN_THREADS];
     pdl_wait();
     pdl_launch_next();
-    const int R = a.nkv * a.row_blocks, group = a.nh / a.nkv, head = blockIdx.y, row = blockIdx.z, tid = threadIdx.x;
+    const int R = a.nkv * a.row_blocks, group = a.nh / a.nkv, row = blockIdx.z, tid = threadIdx.x;
     const int g = row / a.row_blocks, h0 = g * group + row % a.row_blocks * AE_HEADS;
-    if (h0 + head >= (g + 1) * group) return;
-    const int total = all_tiles<AE_JOIN_THREADS>(a, scan, scratch);
-    const int i = blockIdx.x + 1, x = stretch_start(total, i, stretches);
-    if (x >= total) return;
-    int b, begin;
-    find_tile<AE_JOIN_THREADS>(a, x, scan, scratch, b, begin);
-    const int end = begin + seen_by(a, b).tiles;
-    if (x == begin || stretch_start(total, i - 1, stretches) > begin) return;  // not inside, not the first
+    const int i = blockIdx.x + 1;
+    const int4 at = reinterpret_cast<const int4*>(a.partial)[i];               // of the stretch: (sequence, its tiles, all)
+    const int b = at.x, begin = at.y, end = at.z, total = at.w;
+    // (one behind the last tile; one that begins with the sequence; not the first to begin inside it)
+    if (b < 0 || stretch_start(total, i, stretches) == begin || stretch_start(total, i - 1, stretches) > begin) return;
     // the stretches i - 1 .. last have a part of the sequence (but for empty ones)
     const int last = (int)(((long long)end * stretches - 1) / total), parts = last - i + 2;
-    float M = -INFINITY;
-    for (int j = tid; j < parts; j += AE_JOIN_THREADS) {
-        const int part = i - 1 + j, from = stretch_start(total, part, stretches);
-        const int at = from == stretch_start(total, part + 1, stretches) ? -1 : 2 * (part * R + row) + (from < begin);
-        slot[j] = at;
-        weight[j] = at < 0 ? -INFINITY : a.partial[(size_t)at * S::PART + AE_HEADS * DIM + 2 * head];
-        M = fmaxf(M, weight[j]);
-    }
-    M = block_max(M, scratch);
-    const float sink = a.sinks ? a.sinks[h0 + head] * 1.4426950408889634f : -INFINITY;
-    M = fmaxf(M, sink);
-    float L = 0.f;
-    for (int j = tid; j < parts; j += AE_JOIN_THREADS) {
-        const float w = M == -INFINITY ? 1.f : ex2(weight[j] - M);
-        weight[j] = w;
-        if (slot[j] >= 0) L += w * a.partial[(size_t)slot[j] * S::PART + AE_HEADS * DIM + 2 * head + 1];
-    }
-    L = block_sum(L, scratch);                 // (with barriers: the weights are there)
-    if (sink != -INFINITY) L += ex2(sink - M);
-    constexpr int LANES = DIM / 4, GROUPS = AE_JOIN_THREADS / LANES;
-    const int d = tid % LANES * 4;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (d < a.hdv) {
-#pragma unroll 4
-        for (int j = tid / LANES; j < parts; j += GROUPS) {
-            const int at = slot[j];
-            if (at < 0) continue;
-            const float4 u = *reinterpret_cast<const float4*>(a.partial + (size_t)at * S::PART + head * DIM + d);
-            const float w = weight[j];
-            v.x = fmaf(u.x, w, v.x);
-            v.y = fmaf(u.y, w, v.y);
-            v.z = fmaf(u.z, w, v.z);
-            v.w = fmaf(u.w, w, v.w);
+    const float* partial = a.partial + 4 * stretches;
+    for (int head = blockIdx.y; head < AE_HEADS && h0 + head < (g + 1) * group; head += gridDim.y) {
+        __syncthreads();                           // (the head before has been read)
+        float M = -INFINITY;
+        for (int j = tid; j < parts; j += AE_JOIN_THREADS) {
+            const int part = i - 1 + j, from = stretch_start(total, part, stretches);
+            const int at = from == stretch_start(total, part + 1, stretches) ? -1 : 2 * (part * R + row) + (from < begin);
+            slot[j] = at;
+            weight[j] = at < 0 ? -INFINITY : partial[(size_t)at * S::PART + AE_HEADS * DIM + 2 * head];
+            M = fmaxf(M, weight[j]);
         }
-    }
-    sums[tid] = v;
-    __syncthreads();
-    const float* flat = reinterpret_cast<const float*>(sums);
-    T* out = (T*)a.out + ((size_t)b * a.nh + h0 + head) * a.hdv;
-    for (int e = tid; e < a.hdv; e += AE_JOIN_THREADS) {
-        float o = 0.f;
+        M = block_max(M, scratch);
+        const float sink = a.sinks ? a.sinks[h0 + head] * 1.4426950408889634f : -INFINITY;
+        M = fmaxf(M, sink);
+        float L = 0.f;
+        for (int j = tid; j < parts; j += AE_JOIN_THREADS) {
+            const float w = M == -INFINITY ? 1.f : ex2(weight[j] - M);
+            weight[j] = w;
+            if (slot[j] >= 0) L += w * partial[(size_t)slot[j] * S::PART + AE_HEADS * DIM + 2 * head + 1];
+        }
+        L = block_sum(L, scratch);                 // (with barriers: the weights are there)
+        if (sink != -INFINITY) L += ex2(sink - M);
+        constexpr int LANES = DIM / 4, GROUPS = AE_JOIN_THREADS / LANES;
+        const int d = tid % LANES * 4;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (d < a.hdv) {
+#pragma unroll 4
+            for (int j = tid / LANES; j < parts; j += GROUPS) {
+                const int at = slot[j];
+                if (at < 0) continue;
+                const float4 u = *reinterpret_cast<const float4*>(partial + (size_t)at * S::PART + head * DIM + d);
+                const float w = weight[j];
+                v.x = fmaf(u.x, w, v.x);
+                v.y = fmaf(u.y, w, v.y);
+                v.z = fmaf(u.z, w, v.z);
+                v.w = fmaf(u.w, w, v.w);
+            }
+        }
+        sums[tid] = v;
+        __syncthreads();
+        const float* flat = reinterpret_cast<const float*>(sums);
+        T* out = (T*)a.out + ((size_t)b * a.nh + h0 + head) * a.hdv;
+        for (int e = tid; e < a.hdv; e += AE_JOIN_THREADS) {
+            float o = 0.f;
 #pragma unroll
-        for (int q = 0; q < GROUPS; ++q) o += flat[q * DIM + e];
-        out[e] = from_f32<T>(L == 0.f ? 0.f : o / L);
+            for (int q = 0; q < GROUPS; ++q) o += flat[q * DIM + e];
+            out[e] = from_f32<T>(L == 0.f ? 0.f : o / L);
+        }
     }
 }
 
@@ -773,11 +791,16 @@ Plan plan_of(int B, int nh, int nkv, int hd, int hdv, int max_keys) {
     const long long rows = (long long)B * nkv * ((nh / nkv + AE_HEADS - 1) / AE_HEADS);
     const long long tiles = (max_keys + AE_TILE - 1) / AE_TILE + 1;
     const int resident = sm_count() * (p.dim == 256 ? Tile<256>::CTAS : p.dim == 128 ? Tile<128>::CTAS : Tile<64>::CTAS);
-    // A row is the work of a cluster's CTAs where that leaves each a few tiles: one launch, and the
-    // join goes through shared memory.  Else stretches: CTAs for every row there is room for.
+    // A row is the work of a cluster where that leaves each of its CTAs a few tiles: one launch, and the
+    // join goes through shared memory.  As many CTAs as run at a time, 16 only where those are few
+    // (one row of 2000 keys: 32 us with one, 14 with four, 11 with eight, 9.7 with 16; 32 rows of 1000: 19, 12, 11, 26).
+    // Else stretches, which cost the second launch and about 3 us of finding them (4 rows of 4000 keys: 14 us and
+    // 11 with 16 CTAs a row, of 16000: 21 and 23; 256 rows of 1500: 40 and 36 with one CTA a row, of
+    // 4000: 62 and 75).
     p.cluster = 1;
-    while (p.cluster < 16 && p.cluster < tiles && rows * p.cluster * 2 <= resident) p.cluster *= 2;
-    p.split = tiles > 8 * p.cluster;
+    while (p.cluster < 16 && p.cluster < tiles && rows * p.cluster * 2 <= (p.cluster < 8 ? resident : sm_count()))
+        p.cluster *= 2;
+    p.split = tiles > (p.cluster < 8 ? 40 * p.cluster : 240);
     const int R = (int)(rows / B);
     long long stretches = resident / R;                          // all CTAs at a time
     if (stretches > B * tiles) stretches = B * tiles;
@@ -800,9 +823,11 @@ int launch(const AttendE4& a, const Plan& p, cudaStream_t stream) {
     agv_launch_cluster(kern, p.ctas, AE_THREADS, Tile<DIM>::SMEM, stream, dim3(p.split ? 1 : p.cluster), a);
     AGV_LAUNCH_OK("attend_e4m3_kernel");
     if (p.stretches > 1) {
-        const int heads = a.nh / a.nkv < AE_HEADS ? a.nh / a.nkv : AE_HEADS;
-        agv_launch(join_e4m3_kernel<T, DIM>, dim3(p.stretches - 1, heads, a.nkv * a.row_blocks), AE_JOIN_THREADS, 0, stream,
-                   a, p.stretches);
+        // (a CTA a head while that makes no more CTAs than run at a time)
+        const int R = a.nkv * a.row_blocks, heads = a.nh / a.nkv < AE_HEADS ? a.nh / a.nkv : AE_HEADS;
+        const int y = 4 * sm_count() / ((p.stretches - 1) * R);
+        agv_launch(join_e4m3_kernel<T, DIM>, dim3(p.stretches - 1, y < 1 ? 1 : y < heads ? y : heads, R), AE_JOIN_THREADS, 0,
+                   stream, a, p.stretches);
         AGV_LAUNCH_OK("join_e4m3_kernel");
     }
     return 0;
@@ -825,7 +850,7 @@ int launch_dim(const AttendE4& a, const Plan& p, cudaStream_t stream) {
 AGV_API long long agv_attention_decode_e4m3_scratch(int B, int nh, int nkv, int hd, int hdv, int max_keys) {
     AGV_REQUIRE(B >= 0 && nh > 0 && nkv > 0 && nh % nkv == 0, "attention_decode_e4m3: bad sizes (%d query heads over %d)", nh, nkv);
     const Plan p = plan_of(B, nh, nkv, hd, hdv, max_keys);
-    return p.split ? 2ll * p.ctas * (AE_HEADS * p.dim + 2 * AE_HEADS) : 0;
+    return p.split ? 4ll * p.stretches + 2ll * p.ctas * (AE_HEADS * p.dim + 2 * AE_HEADS) : 0;
 }
 
 // One query per batch entry, q [B, nh * hd] (row stride ldq), against the 8-bit cache; out
