@@ -497,6 +497,12 @@ int lp_cluster(int R, int V) {
     return C;
 }
 
+// Threads of a CTA: 512 for few or long rows, else fewer, so that the rows run at a time (an SM takes
+// 1024 threads) and what a CTA does besides reading runs under the others' reads (us with 128, 256 and
+// 512 threads: 300 rows of 32001 24, 17 and 20; 1100 bfloat16 rows of 32001 30, 32 and 42; 3000
+// of 5000 27, 37 and 57; 600 of 100000 78, 65 and 59).
+int lp_threads(long long ctas, int V) { return ctas <= 296 || V > 65536 ? 512 : ctas <= 592 ? 256 : 128; }
+
 template <typename T, bool TOP, int THREADS>
 int lp_launch(const Logprobs& a, int R, cudaStream_t stream) {
     auto kern = logprobs_kernel<T, TOP, THREADS>;
@@ -506,12 +512,10 @@ int lp_launch(const Logprobs& a, int R, cudaStream_t stream) {
 }
 template <typename T>
 int lp_launch(const Logprobs& a, int R, cudaStream_t stream) {
-    // CTAs of 256 threads where there are several short rows for every SM: what a CTA does besides
-    // reading then runs under the others' reads (777 bfloat16 rows of 32001 31 us, 37 with 512
-    // threads; but 600 rows of 100000 65, and 59).
-    const bool small = (long long)R * a.cluster > 296 && a.V <= 65536;
-    if (a.top) return small ? lp_launch<T, true, 256>(a, R, stream) : lp_launch<T, true, 512>(a, R, stream);
-    return small ? lp_launch<T, false, 256>(a, R, stream) : lp_launch<T, false, 512>(a, R, stream);
+    const int threads = lp_threads(R * (long long)a.cluster, a.V);
+    if (threads == 128) return a.top ? lp_launch<T, true, 128>(a, R, stream) : lp_launch<T, false, 128>(a, R, stream);
+    if (threads == 256) return a.top ? lp_launch<T, true, 256>(a, R, stream) : lp_launch<T, false, 256>(a, R, stream);
+    return a.top ? lp_launch<T, true, 512>(a, R, stream) : lp_launch<T, false, 512>(a, R, stream);
 }
 
 }  // namespace
