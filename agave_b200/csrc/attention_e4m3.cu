@@ -14,15 +14,17 @@
 // kv heads of 128: 238 us with stretches that lay along the heads, 191 like this).
 //
 // In a CTA each of four warps takes 16 of a page's positions and runs for itself: its copies
-// (16-byte cp.async, ring of AE_STAGES tiles), its running maximum, its sums; the warps meet only at
+// (16-byte cp.async, a ring of 3 or 4 tiles), its running maximum, its sums; the warps meet only at
 // the end of a row.  Scores are the product K q^T with 16 positions as rows and 8 heads as
 // columns, the sums V^T w with the head's dimensions as rows: e4m3 codes become half floats in
 // registers (exactly), straight in the layout of the matrix instruction, because the order of
 // dimensions along an inner product, and of rows in the result, is free: a thread converts the
-// bytes that it has read 16 at a time.
+// bytes that it has read 16 at a time.  (The conversions, 16 a clock and SM, and the instructions around
+// them are what a warp spends its time on; V's by shifts instead were slower, 281 us against 247.)
+// The next tile's products stand beside a tile's softmax and fill its waits (247 us, 238 with).
 //
 // Precision: codes are exact in half; a query is scaled by a power of two and split into two
-// halves (22 bits) where it is 32-bit, a bfloat16 one fits in one.  Weights are 32-bit, split the same
+// halves (22 bits) where it is 32-bit; a bfloat16 one fits in one.  Weights are 32-bit, split the same
 // way for 32-bit queries and rounded to 11 bits for bfloat16 ones, whose results keep 8.  The
 // scale of a page's values is part of the weights, relative to the greatest one so far and times
 // 2^14: a half holds a weight of up to 2^14 and, 11 bits, down to 2^-14.
@@ -36,7 +38,9 @@ constexpr int AE_THREADS = 32 * AE_WARPS;
 constexpr int AE_TILE = 16 * AE_WARPS;        // positions that a CTA's warps take together
 constexpr int AE_HEADS = 8;                   // query heads of a row
 constexpr int AE_MAX_DIM = 256;
-constexpr float AE_LEAST_SCALE = 7.8886090522101181e-31f;     // 2^-100: what the values' scales are held against at least
+// 2^-100: the values' scales are held against this at least (the factor that brings weights to halves
+// stays finite; of values below 2^-100 * 448 fewer bits come through).
+constexpr float AE_LEAST_SCALE = 7.8886090522101181e-31f;
 
 struct AttendE4 {
     const void* q;
@@ -55,19 +59,13 @@ struct AttendE4 {
 };
 
 // Head sizes are padded with zeros to DIM = 64, 128 or 256.
-#ifdef AE_STAGES_CTAS
-constexpr int ae_sc(int i) { const int v[6] = {S64, C64, S128, C128, S256, C256}; return v[i]; }
-#endif
 template <int DIM>
 struct Tile {
-#ifndef AE_STAGES_CTAS
+    // Tiles of a warp's ring and CTAs resident on an SM: what registers (a row's sums are DIM / 4 of a
+    // thread's) and shared memory allow.  More warps with fewer registers were slower (256: three CTAs
+    // 67 us where two take 61; 128: four 261 us, three 250), more tiles the same.
     static constexpr int STAGES = DIM == 64 ? 4 : 3;
-    static constexpr int CTAS = DIM == 256 ? 2 : DIM == 128 ? 3 : 5;     // resident on an SM
-#else
-
-    static constexpr int STAGES = ae_sc(DIM == 64 ? 0 : DIM == 128 ? 2 : 4);
-    static constexpr int CTAS = ae_sc(DIM == 64 ? 1 : DIM == 128 ? 3 : 5);
-#endif
+    static constexpr int CTAS = DIM == 256 ? 2 : DIM == 128 ? 3 : 5;
     // A warp's 16-byte reads meet every bank once: of two key rows 64 bytes each, which lie in
     // different halves of 128 bytes (odd rows of 128 bytes or more have them exchanged), of four
     // value rows 32 bytes each, by the stride.

@@ -81,6 +81,7 @@ class DecoderModel:
             if not call.writes_cache and call.cache not in writers:
                 raise ValueError(f"cache entry {call.cache} is read but never written")
         self._writers = writers
+        self._borrowed = frozenset(c.cache for c in spec.schedule if not c.writes_cache)
 
     # ----------------------------------------------------------------- cache
     def cache_requests(self) -> List[object]:
@@ -250,6 +251,7 @@ class DecoderModel:
         sched = spec.schedule
         if not sched:
             return h
+        ctx.borrowed_entries = self._borrowed
         start = None                       # the stream before the first block, where it is needed again
         if any(c.add_embedding for c in sched):
             start = ctx.new(T, spec.hidden_size, dtype=torch.float32)

@@ -65,6 +65,14 @@ from .base import KVRequest, ParamSpec, StateRequest, position_class, register_m
 from .linear import Linear
 
 
+def keep_step_kv(ctx, cache_entry: int, kv) -> None:
+    """Holds a prompt step's keys and values for the later calls that read this entry, if there
+    may be any (without them a long prompt's go as soon as the layer is done)."""
+    borrowed = getattr(ctx, "borrowed_entries", None)
+    if borrowed is None or cache_entry in borrowed:
+        ctx.step_kv[cache_entry] = kv
+
+
 class AttentionMixer:
     def __init__(self, spec: AttentionSpec, hidden_size: int, dtype: torch.dtype,
                  device: torch.device):
@@ -467,7 +475,7 @@ class AttentionMixer:
             if self.own_kv:
                 k = qkv[:, nh * hd:(nh + nkv) * hd]
                 v = qkv[:, (nh + nkv) * hd:]
-                ctx.step_kv[cache_entry] = (k, v, vt)
+                keep_step_kv(ctx, cache_entry, (k, v, vt))
             else:
                 k, v, vt = ctx.step_kv[cache_entry]
             kernels.attention_prefill(q, k, v, out, ctx, nh, nkv, hd, s.scale, window, vt=vt,
@@ -527,7 +535,7 @@ class AttentionMixer:
             if self.own_kv:
                 k = qkvg[:, nh * hd:(nh + nkv) * hd]
                 v = qkvg[:, (nh + nkv) * hd:C]
-                ctx.step_kv[cache_entry] = (k, v, None)
+                keep_step_kv(ctx, cache_entry, (k, v, None))
             else:
                 k, v, _ = ctx.step_kv[cache_entry]
             kernels.attention_prefill(q, k, v, out, ctx, nh, nkv, hd, s.scale, window,
@@ -549,7 +557,7 @@ class AttentionMixer:
         if writes_cache:
             k = qkv[:, nh * hd:(nh + nkv) * hd]
             v = qkv[:, (nh + nkv) * hd:]
-            ctx.step_kv[cache_entry] = (k, v, vt)
+            keep_step_kv(ctx, cache_entry, (k, v, vt))
         else:
             k, v, vt = ctx.step_kv[cache_entry]
         out = ctx.new(qkv.shape[0], nh * hd)

@@ -38,6 +38,11 @@ Cases (Gemma 3 1B layer sizes, random bfloat16 data):
   experts_prefill, experts_decode   a routed feed-forward (width 2,048, 32 experts of width
                        768 in 8 groups, 4 of them a token, 4 groups kept): router, plan, gather
                        and the two grouped products, for 2,048 tokens and for 8
+  cache_store_e4m3_prefill   keys and values of 16 prompts of 2,048 tokens (4 kv heads of 256) into the
+                       8-bit cache
+  attention_decode_full_b64_e4m3   decode attention over the 8-bit cache, 64 sequences of 128..8,192
+                       positions, 32 query and 16 kv heads of 128
+  token_logprobs_b64   log-probabilities of 64 rows of 262,144 logits with 20 alternatives
 
 Each case prints the mean time per call: the calls run back to back from a CUDA
 graph, each on the next of several copies of its operands, the copies together
@@ -355,7 +360,61 @@ def case_experts(T):
     return (lambda i: part.forward(x, None)), 6 * T * top * h * ff, nbytes, 1
 
 
+def _e4m3_view(B, length, nkv, hd):
+    from types import SimpleNamespace
+    pages = (length + 63) // 64
+
+    def pool():
+        return _rnd(B * pages, 64, nkv, hd, scale=64.0).to(torch.float8_e4m3fn)
+    scales = torch.full((2, B * pages, nkv), 2.0 ** -6, device=DEV)
+    return SimpleNamespace(
+        k_pool=pool(), v_pool=pool(), k_scale=scales[0], v_scale=scales[1], page=64, cap=pages * 64,
+        page_table=torch.arange(B * pages, dtype=torch.int32, device=DEV).reshape(B, pages), window=None)
+
+
+def _e4m3_ctx(lens, new):
+    from types import SimpleNamespace
+    i = dict(dtype=torch.int32, device=DEV)
+    return SimpleNamespace(
+        slots=torch.arange(len(lens), **i), lens=torch.tensor(lens, **i), max_len=max(lens), mode="decode",
+        positions=torch.tensor([n - 1 for n in lens], **i), max_new=max(new),
+        cu_seqlens=torch.tensor([sum(new[:b]) for b in range(len(new) + 1)], **i))
+
+
+def case_cache_store_e4m3(B=16, length=2048, nkv=4, hd=256):
+    from . import kernels
+    views = [_e4m3_view(B, length, nkv, hd) for _ in range(3)]
+    kv = [_rnd(B * length, 2 * nkv * hd) for _ in range(3)]
+    ctx = _e4m3_ctx([length] * B, [length] * B)
+
+    def fn(i):
+        kernels.cache_store_e4m3(kv[i][:, :nkv * hd], kv[i][:, nkv * hd:], views[i], ctx, nkv, hd)
+    return fn, 0, B * length * 2 * nkv * hd * 3, 3
+
+
+def case_attention_decode_e4m3(B=64, lo=128, hi=8192, nh=32, nkv=16, hd=128):
+    from . import kernels
+    lens = torch.linspace(lo, hi, B).round().int().tolist()
+    view, ctx = _e4m3_view(B, hi, nkv, hd), _e4m3_ctx(lens, [1] * B)
+    q = _rnd(B, nh * hd)
+    out = torch.empty_like(q)
+
+    def fn(i):
+        kernels.attention_decode_e4m3(q, out, view, ctx, nh, nkv, hd, hd ** -0.5, 0)
+    return fn, 0, sum(lens) * nkv * hd * 2, 1
+
+
+def case_token_logprobs(R=64, V=V, top=20):
+    from . import kernels
+    logits = [torch.randn(R, V, device=DEV) * 3 for _ in range(4)]
+    tokens = torch.randint(0, V, (R,), device=DEV).int()
+    return (lambda i: kernels.token_logprobs(logits[i], tokens, top)), 0, R * V * 4, 4
+
+
 CASES = {
+    "cache_store_e4m3_prefill": case_cache_store_e4m3,
+    "attention_decode_full_b64_e4m3": case_attention_decode_e4m3,
+    "token_logprobs_b64": case_token_logprobs,
     "experts_prefill": lambda: case_experts(2048),
     "experts_decode": lambda: case_experts(8),
     "gemm_gated_prefill": lambda: case_gemm_gated(2048),

@@ -67,7 +67,7 @@ def test_store_refuses(lib):
     assert call(B=0)[0] == 0 and call(T=0)[0] == 0
     for kw, word in ((dict(hd=24), "multiples of 16"), (dict(hdv=0), "multiples of 16"), (dict(cap=100), "geometry"),
                      (dict(cap=192), "geometry"), (dict(dtype=2), "dtype"), (dict(pool=8), "unaligned"),
-                     (dict(B=70000), "grid"), (dict(nkv=0), "bad sizes"), (dict(n_slots=0), "bad sizes")):
+                     (dict(B=70000), "grid"), (dict(page=48, cap=96), "geometry"), (dict(nkv=0), "bad sizes"), (dict(n_slots=0), "bad sizes")):
         rc, msg = call(**kw)
         assert rc < 0 and word in msg, (kw, msg)
 

@@ -86,6 +86,23 @@ def test_store_codes_and_scales(dtype, nkv, hd, hdv, counts, lens):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("nkv,hd,hdv,page", [(2, 64, 64, 64), (1, 256, 128, 64), (2, 80, 48, 64), (2, 272, 320, 64),
+                                             (2, 64, 128, 128), (3, 128, 64, 16), (1, 16, 16, 1)])
+@pytest.mark.parametrize("off", [0, 1, 8])
+def test_store_of_rows_anywhere(dtype, nkv, hd, hdv, page, off):
+    """Rows that start on no 16-byte boundary, pages of other sizes, heads wider than attention takes."""
+    view = make_view(4, 256, nkv, hd, hdv, seed=1, page=page)
+    counts, lens = [100, 3, 64, 41], [100, 80, 64, 250]
+    wide = rnd(sum(counts), nkv * (hd + hdv) + 11, dtype=dtype, seed=2, scale=3.0)
+    k, v = wide[:, off:off + nkv * hd], wide[:, off + nkv * hd:off + nkv * (hd + hdv)]
+    check_store(view, make_ctx(counts, lens, [1, 3, 0, 2]), k, v, nkv, hd, hdv)
+    # max_new says less than is brought: the rest is stored all the same
+    ctx = make_ctx(counts, [n + 5 for n in lens], [1, 3, 0, 2])
+    ctx.max_new = 1
+    check_store(view, ctx, k, v, nkv, hd, hdv)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("page", [16, 64])
 def test_store_in_a_ring(dtype, page):
     """A prompt longer than the ring leaves its last pages; then tokens one by one wrap around."""
@@ -211,12 +228,34 @@ def test_attention_in_a_ring(dtype):
 
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("lens,nh,nkv,hd", [([20011], 8, 4, 256), ([9000, 1, 77], 2, 1, 128),
-                                            ([4097] * 3, 16, 8, 64)])
+                                            ([4097] * 3, 16, 8, 64), ([3000] + [50, 700] * 70, 6, 3, 128),
+                                            ([5000] * 2 + [3], 40, 2, 64), ([2500] * 5, 150, 150, 64)])
 def test_attention_of_long_sequences(dtype, lens, nh, nkv, hd):
     cap = (max(lens) + 63) // 64 * 64
     view = make_view(len(lens), cap, nkv, hd, hd, seed=6)
     ctx = make_ctx([1] * len(lens), lens, list(range(len(lens)))[::-1])
     check_attend(view, rnd(len(lens), nh * hd, dtype=dtype, seed=7, scale=2.0), ctx, nh, nkv, hd, hd, hd ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("page", [16, 32, 128])
+@pytest.mark.parametrize("window,keep_first", [(0, 0), (150, 0), (150, 20)])
+def test_attention_with_pages_of_other_sizes(dtype, page, window, keep_first):
+    nh, nkv, hd, lens = 4, 2, 64, [1, 16, 17, 63, 128, 300, 1000, 1024]
+    view = make_view(9, 1024, nkv, hd, hd, seed=7, page=page)
+    ctx = make_ctx([1] * len(lens), lens, [3, 1, 0, 8, 6, 2, 5, 4])
+    q = rnd(len(lens), nh * hd, dtype=dtype, seed=8, scale=2.0)
+    check_attend(view, q, ctx, nh, nkv, hd, hd, hd ** -0.5, window, keep_first=keep_first)
+    # what max_len says sizes the launch, not what is seen
+    for most in (1, 5000, 1 << 20):
+        ctx.max_len = most
+        check_attend(view, q, ctx, nh, nkv, hd, hd, hd ** -0.5, window, keep_first=keep_first)
+    # a sequence without a key: zeros
+    ctx.positions[2] = -1
+    out = torch.full((len(lens), nh * hd), math.nan, dtype=dtype, device=DEV)
+    from agave_b200 import kernels
+    kernels.attention_decode_e4m3(q, out, view, ctx, nh, nkv, hd, hd ** -0.5, window)
+    assert (out[2] == 0).all() and torch.isfinite(out).all()
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
