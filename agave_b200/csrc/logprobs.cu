@@ -70,24 +70,25 @@ struct Sums {
         s *= f;
         c = to;
     }
-    __device__ __forceinline__ void join(float oc, float os, float ot) {
-        Sums o{oc, os, ot};
-        const float to = fmaxf(c, o.c);
-        if (to == -INFINITY) {                    // (only NaN may be in them)
-            s += o.s;
-            return;
-        }
-        move(to);
-        o.move(to);
-        s += o.s;
-        t += o.t;
-    }
 };
+// Sums of WIDTH neighbouring lanes (a power of two), all relative to their greatest reference, in every one.
+template <int WIDTH>
+__device__ __forceinline__ void join_lanes(Sums& a) {
+    float to = a.c;
+#pragma unroll
+    for (int o = WIDTH / 2; o > 0; o >>= 1) to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, o));
+    if (to != -INFINITY) a.move(to);               // (else nothing but NaN can be in them)
+#pragma unroll
+    for (int o = WIDTH / 2; o > 0; o >>= 1) {
+        a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+        a.t += __shfl_xor_sync(0xffffffffu, a.t, o);
+    }
+}
 
 struct Logprobs {
     const void* logits;
     long long ld;
-    int V, top, cluster;
+    int V, top, cluster_bits;                  // 2^cluster_bits CTAs a row
     const int* tokens;
     float *logprob, *entropy;
     int* rank;
@@ -201,16 +202,16 @@ __global__ void __launch_bounds__(LP_THREADS, 1024 / LP_THREADS) logprobs_kernel
     __shared__ u64 warp_best[TOP ? LP_WARPS : 1];
     __shared__ int n_list;
     __shared__ u64 bound_key;
-    const int C = a.cluster;
+    const int C = 1 << a.cluster_bits;
     if (C > 1) lp_cluster_arrive();                        // (a CTA's memory is written to once it runs)
     pdl_wait();
     pdl_launch_next();
-    const int row = blockIdx.x / C, rank = C > 1 ? (int)lp_cluster_rank() : 0;
+    const int row = blockIdx.x >> a.cluster_bits, rank = C > 1 ? (int)lp_cluster_rank() : 0;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const T* x = (const T*)a.logits + (long long)row * a.ld;
     // the row as 16-byte pieces behind a head that ends at a 16-byte boundary
     const int head = min(a.V, (int)((16 - (uintptr_t)x % 16) % 16 / sizeof(T)));
-    const int pieces = (a.V - head) / N, per = (pieces + C - 1) / C;
+    const int pieces = (a.V - head) / N, per = (pieces + C - 1) >> a.cluster_bits;
     const int v0 = min(pieces, rank * per), v1 = min(pieces, v0 + per);
     const T* body = x + head;
 
@@ -331,12 +332,7 @@ __global__ void __launch_bounds__(LP_THREADS, 1024 / LP_THREADS) logprobs_kernel
         ahead += xe > xt || (xe == xt && edge < tok);
     }
     // ---- sums and counts of the CTA
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float oc = __shfl_xor_sync(0xffffffffu, sum.c, o), os = __shfl_xor_sync(0xffffffffu, sum.s, o);
-        const float ot = __shfl_xor_sync(0xffffffffu, sum.t, o);
-        sum.join(oc, os, ot);
-    }
+    join_lanes<32>(sum);
     ahead = __reduce_add_sync(0xffffffffu, ahead);
     if (lane == 0) {
         wsum[warp] = sum;
@@ -361,13 +357,9 @@ __global__ void __launch_bounds__(LP_THREADS, 1024 / LP_THREADS) logprobs_kernel
     if (warp == LP_WARPS - 1) {
         Sums all = wsum[lane & (LP_WARPS - 1)];
         int n = wahead[lane & (LP_WARPS - 1)];
+        join_lanes<LP_WARPS>(all);
 #pragma unroll
-        for (int o = LP_WARPS / 2; o > 0; o >>= 1) {
-            const float oc = __shfl_xor_sync(0xffffffffu, all.c, o), os = __shfl_xor_sync(0xffffffffu, all.s, o);
-            const float ot = __shfl_xor_sync(0xffffffffu, all.t, o);
-            all.join(oc, os, ot);
-            n += __shfl_xor_sync(0xffffffffu, n, o);
-        }
+        for (int o = LP_WARPS / 2; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
         sum = all;                                         // handed on below
         ahead = n;
     }
@@ -450,12 +442,17 @@ __global__ void __launch_bounds__(LP_THREADS, 1024 / LP_THREADS) logprobs_kernel
         __syncthreads();
     }
     if (rank != 0) return;
-    Sums all{slices[0].c, slices[0].s, slices[0].t};
-    int n_ahead = slices[0].ahead;
-    for (int r = 1; r < C; ++r) {
-        all.join(slices[r].c, slices[r].s, slices[r].t);
-        n_ahead += slices[r].ahead;
+    // (every warp for itself: lane r has slice r's)
+    Sums all{-INFINITY, 0.f, 0.f};
+    int n_ahead = 0;
+    if ((lane & (LP_MAX_CLUSTER - 1)) < C) {
+        const Slice& from = slices[lane & (LP_MAX_CLUSTER - 1)];
+        all = Sums{from.c, from.s, from.t};
+        n_ahead = from.ahead;
     }
+    join_lanes<LP_MAX_CLUSTER>(all);
+#pragma unroll
+    for (int o = LP_MAX_CLUSTER / 2; o > 0; o >>= 1) n_ahead += __shfl_xor_sync(0xffffffffu, n_ahead, o);
     const float nan = __uint_as_float(0x7fffffffu);
     const float ls = all.s > 0.f ? logf(all.s) : nan;     // (no softmax: NaN, or nothing but -inf)
     if (tid == 0) {
@@ -491,10 +488,10 @@ __global__ void __launch_bounds__(LP_THREADS, 1024 / LP_THREADS) logprobs_kernel
 // CTAs for a row: as many, up to 8, as leave slices of some thousand logits and at most about the 296 CTAs
 // of 512 threads that run at a time (64 rows of 262144: 35 us with one CTA a row, 23 with two, 22
 // with four, 35 with eight; one row: 27, 18, 13, 11; 64 rows of 32001: 9.2, 8.7, 10.3, 19).
-int lp_cluster(int R, int V) {
-    int C = 1;
-    while (C < 8 && (long long)R * C * 2 <= 296 && V >= C * 2 * 8000) C *= 2;
-    return C;
+int lp_cluster_bits(int R, int V) {
+    int bits = 0;
+    while (bits < 3 && (long long)R << (bits + 1) <= 296 && V >> (bits + 1) >= 8000) ++bits;
+    return bits;
 }
 
 // Threads of a CTA: 512 for few or long rows, else fewer, so that the rows run at a time (an SM takes
@@ -506,13 +503,14 @@ int lp_threads(long long ctas, int V) { return ctas <= 296 || V > 65536 ? 512 : 
 template <typename T, bool TOP, int THREADS>
 int lp_launch(const Logprobs& a, int R, cudaStream_t stream) {
     auto kern = logprobs_kernel<T, TOP, THREADS>;
-    agv_launch_cluster(kern, dim3((unsigned)(R * a.cluster)), THREADS, 0, stream, dim3(a.cluster), a);
+    agv_launch_cluster(kern, dim3((unsigned)R << a.cluster_bits), THREADS, 0, stream,
+                       dim3(1u << a.cluster_bits), a);
     AGV_LAUNCH_OK("logprobs_kernel");
     return 0;
 }
 template <typename T>
 int lp_launch(const Logprobs& a, int R, cudaStream_t stream) {
-    const int threads = lp_threads(R * (long long)a.cluster, a.V);
+    const int threads = lp_threads((long long)R << a.cluster_bits, a.V);
     if (threads == 128) return a.top ? lp_launch<T, true, 128>(a, R, stream) : lp_launch<T, false, 128>(a, R, stream);
     if (threads == 256) return a.top ? lp_launch<T, true, 256>(a, R, stream) : lp_launch<T, false, 256>(a, R, stream);
     return a.top ? lp_launch<T, true, 512>(a, R, stream) : lp_launch<T, false, 512>(a, R, stream);
@@ -531,8 +529,6 @@ AGV_API int agv_token_logprobs(const void* logits, long long ld, int dtype, int 
                 V < LP_MAX_TOP ? V : LP_MAX_TOP);
     AGV_REQUIRE(dtype == AGV_F32 || dtype == AGV_BF16, "token_logprobs: bad dtype");
     if (R == 0) return 0;
-    const int C = lp_cluster(R, V);
-    AGV_REQUIRE((long long)R * C <= 0x7fffffffLL, "token_logprobs: %d rows exceed the grid", R);
-    Logprobs a{logits, ld, V, top, C, tokens, logprob, entropy, rank, top_ids, top_logprobs};
+    Logprobs a{logits, ld, V, top, lp_cluster_bits(R, V), tokens, logprob, entropy, rank, top_ids, top_logprobs};
     return dtype == AGV_F32 ? lp_launch<float>(a, R, stream) : lp_launch<__nv_bfloat16>(a, R, stream);
 }
