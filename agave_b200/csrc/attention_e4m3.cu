@@ -19,8 +19,8 @@
 // columns, the sums V^T w with the head's dimensions as rows: e4m3 codes become half floats in
 // registers (exactly), straight in the layout of the matrix instruction, because the order of
 // dimensions along an inner product, and of rows in the result, is free: a thread converts the
-// bytes that it has read 16 at a time.  (The conversions, 16 a clock and SM, and the instructions around
-// them are what a warp spends its time on; V's by shifts instead were slower, 281 us against 247.)
+// bytes that it has read 16 at a time.  (The conversions run on the integer pipe and are the most of
+// what keeps it half busy; V's by shifts instead were slower, 281 us against 247.)
 // The next tile's products stand beside a tile's softmax and fill its waits (247 us, 238 with).
 //
 // Precision: codes are exact in half; a query is scaled by a power of two and split into two

@@ -496,9 +496,11 @@ int lp_cluster_bits(int R, int V) {
 
 // Threads of a CTA: 512 for few or long rows, else fewer, so that the rows run at a time (an SM takes
 // 1024 threads) and what a CTA does besides reading runs under the others' reads (us with 128, 256 and
-// 512 threads: 300 rows of 32001 24, 17 and 20; 1100 bfloat16 rows of 32001 30, 32 and 42; 3000
-// of 5000 27, 37 and 57; 600 of 100000 78, 65 and 59).
-int lp_threads(long long ctas, int V) { return ctas <= 296 || V > 65536 ? 512 : ctas <= 592 ? 256 : 128; }
+// 512 threads: 300 rows of 32001 24, 17 and 20; 777 bfloat16 rows of 32001 26.5, 24.6 and 33, 1100 30, 32
+// and 42; 1000 rows of 5000 12, 15 and 21; 600 of 100000 78, 65 and 59).
+int lp_threads(long long ctas, int V) {
+    return ctas <= 296 || V > 65536 ? 512 : ctas <= (V > 8192 ? 1000 : 592) ? 256 : 128;
+}
 
 template <typename T, bool TOP, int THREADS>
 int lp_launch(const Logprobs& a, int R, cudaStream_t stream) {

@@ -2121,8 +2121,8 @@ def cache_store_e4m3(k: torch.Tensor, v: torch.Tensor, view, ctx, n_kv_heads: in
     cu, slots, lens = ctx.cu_seqlens, ctx.slots, ctx.lens
     kp, vp, ks, vs, table = view.k_pool, view.v_pool, view.k_scale, view.v_scale, view.page_table
     dev = _raw_device() if _raw_device is not None else torch.cuda.current_device()
-    T, B = len(k), len(slots)
-    pages, page = len(kp), view.page
+    T, B = k.shape[0], slots.numel()
+    pages, page = kp.shape[0], view.page
     scales = (pages, n_kv_heads)
     # (all at once: a call of one token is mostly its checks)
     if not (dev == k.get_device() == v.get_device() == kp.get_device() == vp.get_device() ==
@@ -2175,7 +2175,7 @@ def attention_decode_e4m3(q: torch.Tensor, out: torch.Tensor, view, ctx, n_heads
         raise KernelError(f"attention_decode_e4m3: head sizes {head_dim} and {hdv} must be multiples "
                           f"of 16 up to {E4M3_MAX_HEAD}")
     dev = _raw_device() if _raw_device is not None else torch.cuda.current_device()
-    B, pages, page = len(q), len(kp), view.page
+    B, pages, page = q.shape[0], kp.shape[0], view.page
     scales = (pages, n_kv_heads)
     dtype = q.dtype
     if not (dev == q.get_device() == out.get_device() == kp.get_device() == vp.get_device() ==
