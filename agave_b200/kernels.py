@@ -2047,6 +2047,7 @@ def attention_decode(q, out, view, ctx, n_heads, n_kv_heads, head_dim, scale, wi
 # --------------------------------------------------------------- the 8-bit cache
 E4M3 = torch.float8_e4m3fn
 E4M3_MAX_HEAD = 256
+_E4M3_NO_SCRATCH_KEYS = 1024        # up to so many keys no size wants scratch (the C function would say 0)
 
 
 def e4m3_head_supported(head_dim: int, value_dim: int = 0) -> bool:
@@ -2211,9 +2212,11 @@ def attention_decode_e4m3(q: torch.Tensor, out: torch.Tensor, view, ctx, n_heads
         bias_at, n_dist = dist_bias.data_ptr(), dist_bias.shape[1]
     max_keys = max(1, min(abs(window) + keep_first, ctx.max_len) if window else ctx.max_len)
     lib = _lib or library()
-    floats = lib.agv_attention_decode_e4m3_scratch(B, n_heads, n_kv_heads, head_dim, hdv, max_keys)
-    if floats < 0:
-        _check(floats)
+    floats = 0
+    if max_keys > _E4M3_NO_SCRATCH_KEYS or n_heads % n_kv_heads:
+        floats = lib.agv_attention_decode_e4m3_scratch(B, n_heads, n_kv_heads, head_dim, hdv, max_keys)
+        if floats < 0:
+            _check(floats)
     partial = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
     with _span(op, *_attention_cost(ctx, q, None, None, out, n_heads, head_dim, window, n_kv_heads,
                                     1)) if _perf is not None or NVTX else _UNWATCHED:
@@ -2276,15 +2279,15 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
         raise KernelError(f"token_logprobs: top {top} must lie in 0..{min(V, LOGPROBS_MAX_TOP)}")
     r = None
     if packed is None:
-        r, new, f32, i32, on = TokenLogprobs(), torch.empty, torch.float32, torch.int32, logits.device
-        r.logprob = a = new(R, dtype=f32, device=on)
-        r.entropy = b = new(R, dtype=f32, device=on)
-        r.rank = c = new(R, dtype=i32, device=on)
+        r, new, f32 = TokenLogprobs(), tokens.new_empty, torch.float32
+        r.logprob = a = new(R, dtype=f32)
+        r.entropy = b = new(R, dtype=f32)
+        r.rank = c = new(R)
         r.top_ids = r.top_logprobs = None
         out = (a.data_ptr(), b.data_ptr(), c.data_ptr(), None, None)
         if top:
-            r.top_ids = a = new((R, top), dtype=i32, device=on)
-            r.top_logprobs = b = new((R, top), dtype=f32, device=on)
+            r.top_ids = a = new((R, top))
+            r.top_logprobs = b = new((R, top), dtype=f32)
             out = out[:3] + (a.data_ptr(), b.data_ptr())
     else:
         _on_current_device(packed); _f32(packed, "packed")
