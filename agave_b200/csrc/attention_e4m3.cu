@@ -324,10 +324,9 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
         const int n = min(s.tiles - tile, left);                     // tiles of this segment
         const bool whole = n == s.tiles;
         if (s.slot < 0) {
-            if (!shared_row || left > 0) {
+            // padding (of a cluster the CTA that has its one tile)
             T* out = (T*)a.out + ((size_t)b * a.nh + h0) * a.hdv;
-            for (int i = tid; i < heads * a.hdv; i += AE_THREADS) out[i] = from_f32<T>(0.f);
-            }
+            for (int i = tid; i < heads * a.hdv && left > 0; i += AE_THREADS) out[i] = from_f32<T>(0.f);
         } else {
             const int* table = a.table + (size_t)s.slot * a.max_pages;
             const size_t krow = (size_t)a.nkv * a.hd, vrow = (size_t)a.nkv * a.hdv;
@@ -359,7 +358,8 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
             constexpr int LPR = DIM / 16, RPI = 32 / LPR;        // lanes a row, rows an instruction
             const int crow = lane / LPR, ccol = lane % LPR * 16;
             const int flip = DIM > 64 ? (crow & 1) * 64 : 0;
-            const unsigned copy_at = mine_at + crow * S::KS + (ccol ^ flip), copy_vat = mine_at + 16 * S::KS + crow * S::VS + ccol;
+            const unsigned copy_at = mine_at + crow * S::KS + (ccol ^ flip);
+            const unsigned copy_vat = mine_at + 16 * S::KS + crow * S::VS + ccol;
             const int k_bytes = ccol < a.hd ? 16 : 0, v_bytes = ccol < a.hdv ? 16 : 0;
             const unsigned char* k_from = a.k_pool + (size_t)crow * krow + (size_t)g * a.hd + (k_bytes ? ccol : 0);
             const unsigned char* v_from = a.v_pool + (size_t)crow * vrow + (size_t)g * a.hdv + (v_bytes ? ccol : 0);
@@ -593,8 +593,10 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
                     }
 #pragma unroll
                     for (int f = 0; f < VB / 4; ++f) {
-                        const unsigned la = __byte_perm(w[0][f], w[1][f], 0x5140), lb = __byte_perm(w[0][f], w[1][f], 0x7362);
-                        const unsigned ha = __byte_perm(w[2][f], w[3][f], 0x5140), hb = __byte_perm(w[2][f], w[3][f], 0x7362);
+                        const unsigned la = __byte_perm(w[0][f], w[1][f], 0x5140);
+                        const unsigned lb = __byte_perm(w[0][f], w[1][f], 0x7362);
+                        const unsigned ha = __byte_perm(w[2][f], w[3][f], 0x5140);
+                        const unsigned hb = __byte_perm(w[2][f], w[3][f], 0x7362);
                         const int t = q * (VB / 2) + 2 * f;
                         unsigned a0, a1, a2, a3;
                         e4m3_word(la, a0, a1);
@@ -651,7 +653,8 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
                 }
             }
             __syncthreads();
-            float* part = a.partial ? a.partial + gridDim.x / R * 4 + (size_t)(2 * blockIdx.x + (segment > 0)) * S::PART : nullptr;
+            float* part = nullptr;
+            if (a.partial) part = a.partial + gridDim.x / R * 4 + (size_t)(2 * blockIdx.x + (segment > 0)) * S::PART;
             if (shared_row) {
                 share_row<T, DIM>(a, red, stat, b, h0, heads);
                 return;
@@ -695,8 +698,8 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
 }
 
 // ---------------------------------------------------------------- rows of several CTAs
-// CTA (i, h, r) joins, for head h of 8 of row r (and every gridDim.y-th after it), the sequence inside which stretch i + 1 begins, if it
-// is the first to begin there.  First the partial results' weights, a thread each, then the sums:
+// CTA (i, h, r) joins, for head h of 8 of row r (and every gridDim.y-th after it), the sequence inside
+// which stretch i + 1 begins, if it is the first to begin there.  First the partial results' weights, a thread each, then the sums:
 // DIM / 4 threads take a partial result, the CTA 8 to 32 of them at a time.
 constexpr int AE_JOIN_THREADS = 512;
 constexpr int AE_MAX_STRETCHES = 1024;
@@ -789,7 +792,8 @@ Plan plan_of(int B, int nh, int nkv, int hd, int hdv, int max_keys) {
     Plan p;
     const int most = hd > hdv ? hd : hdv;
     p.dim = most <= 64 ? 64 : most <= 128 ? 128 : 256;
-    const long long rows = (long long)B * nkv * ((nh / nkv + AE_HEADS - 1) / AE_HEADS);
+    const int R = nkv * ((nh / nkv + AE_HEADS - 1) / AE_HEADS);
+    const long long rows = (long long)B * R;
     const long long tiles = (max_keys + AE_TILE - 1) / AE_TILE + 1;
     const int resident = sm_count() * (p.dim == 256 ? Tile<256>::CTAS : p.dim == 128 ? Tile<128>::CTAS : Tile<64>::CTAS);
     // A row is the work of a cluster where that leaves each of its CTAs a few tiles: one launch, and the
@@ -802,7 +806,6 @@ Plan plan_of(int B, int nh, int nkv, int hd, int hdv, int max_keys) {
     while (p.cluster < 16 && p.cluster < tiles && rows * p.cluster * 2 <= (p.cluster < 8 ? resident : sm_count()))
         p.cluster *= 2;
     p.split = tiles > (p.cluster < 8 ? 40 * p.cluster : 240);
-    const int R = (int)(rows / B);
     long long stretches = resident / R;                          // all CTAs at a time
     if (stretches > B * tiles) stretches = B * tiles;
     if (stretches > AE_MAX_STRETCHES) stretches = AE_MAX_STRETCHES;
@@ -849,7 +852,8 @@ int launch_dim(const AttendE4& a, const Plan& p, cudaStream_t stream) {
 
 // 32-bit values of scratch that agv_attention_decode_e4m3 wants for these sizes.
 AGV_API long long agv_attention_decode_e4m3_scratch(int B, int nh, int nkv, int hd, int hdv, int max_keys) {
-    AGV_REQUIRE(B >= 0 && nh > 0 && nkv > 0 && nh % nkv == 0, "attention_decode_e4m3: bad sizes (%d query heads over %d)", nh, nkv);
+    AGV_REQUIRE(B >= 0 && nh > 0 && nkv > 0 && nh % nkv == 0,
+                "attention_decode_e4m3: bad sizes (%d query heads over %d)", nh, nkv);
     const Plan p = plan_of(B, nh, nkv, hd, hdv, max_keys);
     return p.split ? 4ll * p.stretches + 2ll * p.ctas * (AE_HEADS * p.dim + 2 * AE_HEADS) : 0;
 }
@@ -879,7 +883,8 @@ AGV_API int agv_attention_decode_e4m3(const void* q, long long ldq, void* out, i
     AGV_REQUIRE(keep_first >= 0 && softcap >= 0.f && (!dist_bias || n_dist > 0), "attention_decode_e4m3: bad options");
     if (B == 0) return 0;
     const Plan plan = plan_of(B, nh, nkv, hd, hdv, max_keys);
-    AGV_REQUIRE(!plan.split || (partial && agv_aligned(partial, 16) && partial_floats >= agv_attention_decode_e4m3_scratch(B, nh, nkv, hd, hdv, max_keys)),
+    const long long wanted = agv_attention_decode_e4m3_scratch(B, nh, nkv, hd, hdv, max_keys);
+    AGV_REQUIRE(!plan.split || (partial && agv_aligned(partial, 16) && partial_floats >= wanted),
                 "attention_decode_e4m3: %lld floats of scratch are too few", partial_floats);
     const size_t esz = dtype == AGV_F32 ? 4 : 2;
     int page_bits = 0;

@@ -126,7 +126,8 @@ __device__ __forceinline__ unsigned e4m3_quad_finite(float a, float b, float c, 
 
 // WHOLE: the pieces of a row are a power of two, so a thread's pieces are all in one column.
 template <typename T, int PIECES, int THREADS, bool WHOLE>
-__global__ void __launch_bounds__(THREADS, (WHOLE || THREADS > 256 ? 1024 : 768) / THREADS) store_pages_e4m3_kernel(const StoreE4 a) {
+__global__ void __launch_bounds__(THREADS, (WHOLE || THREADS > 256 ? 1024 : 768) / THREADS)
+store_pages_e4m3_kernel(const StoreE4 a) {
     constexpr int N = 16 / sizeof(T);
     pdl_wait();
     pdl_launch_next();
@@ -206,8 +207,10 @@ __global__ void __launch_bounds__(THREADS, (WHOLE || THREADS > 256 ? 1024 : 768)
                     float x[N];
                     piece_values<T>(u[i], x);
                     const unsigned w = codes(x[0], x[1], x[2], x[3], any);
-                    if constexpr (N == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w, codes(x[N - 4], x[N - 3], x[N - 2], x[N - 1], any));
-                    else *reinterpret_cast<unsigned*>(dst) = w;
+                    if constexpr (N == 8)
+                        *reinterpret_cast<uint2*>(dst) = make_uint2(w, codes(x[N - 4], x[N - 3], x[N - 2], x[N - 1], any));
+                    else
+                        *reinterpret_cast<unsigned*>(dst) = w;
                 }
                 r += row_step;
                 c += col_step;
@@ -271,8 +274,8 @@ AGV_API int agv_cache_store_e4m3(const void* k, long long ldk, const void* v, lo
     const dim3 grid(nkv, blocks < 65535 ? blocks : 65535, 2 * B);
     const size_t esz = dtype == AGV_F32 ? 4 : 2;
     const int most_dim = hd > hdv ? hd : hdv;
-    if (most > 1 && page <= 64 && most_dim <= 256 && (long long)page * nkv * most_dim <= 0x7fffffff && agv_aligned(k, 16) && agv_aligned(v, 16) && ldk * esz % 16 == 0 &&
-        ldv * esz % 16 == 0) {
+    if (most > 1 && page <= 64 && most_dim <= 256 && (long long)page * nkv * most_dim <= 0x7fffffff &&
+        agv_aligned(k, 16) && agv_aligned(v, 16) && ldk * esz % 16 == 0 && ldv * esz % 16 == 0) {
         if (dtype == AGV_F32) launch_pages<float>(a, grid, stream);
         else launch_pages<__nv_bfloat16>(a, grid, stream);
         AGV_LAUNCH_OK("store_pages_e4m3_kernel");

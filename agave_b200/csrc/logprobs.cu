@@ -177,11 +177,17 @@ template <> struct Piece<__nv_bfloat16> {
     static __device__ __forceinline__ f32x2 above(const uint4& u, float than, bool or_equal) {
         const __nv_bfloat162 b = __float2bfloat162_rn(than);      // (a logit's own value: exact)
         __nv_bfloat162 n;
-        if (or_equal) n = __hadd2(__hadd2(__hge2(pair(u.x), b), __hge2(pair(u.y), b)), __hadd2(__hge2(pair(u.z), b), __hge2(pair(u.w), b)));
-        else n = __hadd2(__hadd2(__hgt2(pair(u.x), b), __hgt2(pair(u.y), b)), __hadd2(__hgt2(pair(u.z), b), __hgt2(pair(u.w), b)));
+        if (or_equal)
+            n = __hadd2(__hadd2(__hge2(pair(u.x), b), __hge2(pair(u.y), b)),
+                        __hadd2(__hge2(pair(u.z), b), __hge2(pair(u.w), b)));
+        else
+            n = __hadd2(__hadd2(__hgt2(pair(u.x), b), __hgt2(pair(u.y), b)),
+                        __hadd2(__hgt2(pair(u.z), b), __hgt2(pair(u.w), b)));
         return pack2(__low2float(n), __high2float(n));
     }
-    static __device__ __forceinline__ __nv_bfloat162 pair(unsigned w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); }
+    static __device__ __forceinline__ __nv_bfloat162 pair(unsigned w) {
+        return *reinterpret_cast<const __nv_bfloat162*>(&w);
+    }
     static __device__ __forceinline__ float greatest(const uint4& u) {
         const __nv_bfloat162 m = __hmax2(__hmax2(pair(u.x), pair(u.y)), __hmax2(pair(u.z), pair(u.w)));
         return fmaxf(__low2float(m), __high2float(m));

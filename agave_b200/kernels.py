@@ -2213,7 +2213,7 @@ def attention_decode_e4m3(q: torch.Tensor, out: torch.Tensor, view, ctx, n_heads
     max_keys = max(1, min(abs(window) + keep_first, ctx.max_len) if window else ctx.max_len)
     lib = _lib or library()
     floats = 0
-    if max_keys > _E4M3_NO_SCRATCH_KEYS or n_heads % n_kv_heads:
+    if max_keys > _E4M3_NO_SCRATCH_KEYS or n_kv_heads < 1 or n_heads % n_kv_heads:
         floats = lib.agv_attention_decode_e4m3_scratch(B, n_heads, n_kv_heads, head_dim, hdv, max_keys)
         if floats < 0:
             _check(floats)

@@ -477,3 +477,5 @@ def test_refusals():
                            positions=ctx.positions[:0], max_new=0, max_len=0, mode="decode")
     store(k[:0], k[:0], view, none, nkv, hd)
     attend(q[:0], out[:0], view, none, nh, nkv, hd, 1.0, 0)
+    none.max_len = 1 << 20
+    attend(q[:0], out[:0], view, none, nh, nkv, hd, 1.0, 0)
