@@ -794,7 +794,7 @@ Plan plan_of(int B, int nh, int nkv, int hd, int hdv, int max_keys) {
     p.dim = most <= 64 ? 64 : most <= 128 ? 128 : 256;
     const int R = nkv * ((nh / nkv + AE_HEADS - 1) / AE_HEADS);
     const long long rows = (long long)B * R;
-    const long long tiles = (max_keys + AE_TILE - 1) / AE_TILE + 1;
+    const long long tiles = ((long long)max_keys + AE_TILE - 1) / AE_TILE + 1;
     const int resident = sm_count() * (p.dim == 256 ? Tile<256>::CTAS : p.dim == 128 ? Tile<128>::CTAS : Tile<64>::CTAS);
     // A row is the work of a cluster where that leaves each of its CTAs a few tiles: one launch, and the
     // join goes through shared memory.  As many CTAs as run at a time, 16 only where those are few

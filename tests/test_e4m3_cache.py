@@ -89,7 +89,8 @@ def test_attention_refuses(lib):
         assert lib.agv_attention_decode_e4m3_scratch(0, 4, 2, 64, 64, keys) >= 0
     for B, nh, nkv, hd in ((1, 1, 1, 16), (1, 128, 128, 256), (3, 40, 2, 64), (2000, 16, 16, 128)):
         assert lib.agv_attention_decode_e4m3_scratch(B, nh, nkv, hd, hd, 1024) == 0
-    assert lib.agv_attention_decode_e4m3_scratch(1, 4, 4, 64, 64, 1 << 20) > 0
+    for keys in (1 << 20, (1 << 31) - 1):
+        assert lib.agv_attention_decode_e4m3_scratch(1, 4, 4, 64, 64, keys) > 0
     for nh, nkv in ((5, 2), (4, 0), (0, 1)):
         assert lib.agv_attention_decode_e4m3_scratch(1, nh, nkv, 64, 64, 4096) < 0
     for kw, word in ((dict(hd=272), "multiples of 16"), (dict(hdv=8), "multiples of 16"), (dict(cap=192), "geometry"),
