@@ -25,9 +25,14 @@
 //
 // Precision: codes are exact in half; a query is scaled by a power of two and split into two
 // halves (22 bits) where it is 32-bit; a bfloat16 one fits in one.  Weights are 32-bit, split the same
-// way for 32-bit queries and rounded to 11 bits for bfloat16 ones, whose results keep 8.  The
-// scale of a page's values is part of the weights, relative to the greatest one so far and times
-// 2^14: a half holds a weight of up to 2^14 and, 11 bits, down to 2^-14.
+// way for 32-bit queries and rounded to 11 bits for bfloat16 ones, whose results keep 8.  The scale 2^e
+// of a page's values is part of the weights that are multiplied with them: the products e^s 2^e have
+// a reference of their own, the greatest so far, apart from the maximum of the scores, which the
+// normaliser goes by (so a page with a great scale and no weight takes no bits from the others).
+// Against it and times 2^14 a half holds a product of up to 2^14 and, 11 bits, down to 2^-14; what is
+// smaller is off by 2^-39 of the greatest.  A warp's sums are divided by the normaliser before they
+// leave their reference: they are values again, in 32 bits as those are, and joining them
+// takes nothing but the maxima and normalisers.
 #include "e4m3.cuh"
 #include <atomic>
 
@@ -38,9 +43,6 @@ constexpr int AE_THREADS = 32 * AE_WARPS;
 constexpr int AE_TILE = 16 * AE_WARPS;        // positions that a CTA's warps take together
 constexpr int AE_HEADS = 8;                   // query heads of a row
 constexpr int AE_MAX_DIM = 256;
-// 2^-100: the values' scales are held against this at least (the factor that brings weights to halves
-// stays finite; of values below 2^-100 * 448 fewer bits come through).
-constexpr float AE_LEAST_SCALE = 7.8886090522101181e-31f;
 
 struct AttendE4 {
     const void* q;
@@ -74,7 +76,7 @@ struct Tile {
     static constexpr int RED = DIM + 4;                                   // floats
     static constexpr int SMEM = AE_WARPS * STAGES * STAGE;
     static_assert(SMEM >= AE_WARPS * AE_HEADS * RED * 4, "the join of the warps uses the same memory");
-    // a partial result: sums [8][DIM], then (maximum, normaliser) of the 8 heads
+    // a partial result: outputs [8][DIM], then (maximum, normaliser) of the 8 heads
     static constexpr int PART = AE_HEADS * DIM + 2 * AE_HEADS;
 };
 
@@ -82,6 +84,14 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// 2^(d + e) for d <= 0 and a whole number e as two factors, neither of which leaves the range where their
+// product with something does not; d = -inf: 0.
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((unsigned)(max(e, -126) + 127) << 23); }
+__device__ __forceinline__ float2 two_factors(float d, float e) {
+    const float whole = fmaxf(rintf(d), -500.f);
+    const int t = (int)(whole + e), half = t >> 1;
+    return make_float2(power_of_two(half), ex2(d - whole) * power_of_two(t - half));
 }
 __device__ __forceinline__ unsigned half2_of(float lo, float hi) {
     unsigned r;
@@ -217,14 +227,14 @@ __device__ __forceinline__ float peer_f32(const void* mine, int rank) {
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
     return v;
 }
-// The CTAs of a cluster join their results for a row: each brings its warps' sums together in its
-// own shared memory, and writes its share of the output from everybody's.
+// The CTAs of a cluster join their results for a row: each brings its warps' outputs together in its
+// own shared memory, and writes its share of the row's from everybody's.  ml: the maximum and normaliser
+// of each head in this CTA.
 template <typename T, int DIM>
-__device__ __forceinline__ void share_row(const AttendE4& a, float* red, float (*stat)[AE_HEADS][2], int b, int h0,
+__device__ __forceinline__ void share_row(const AttendE4& a, float* red, const float (*ml)[2], int b, int h0,
                                           int heads) {
     using S = Tile<DIM>;
-    __shared__ float ml[AE_HEADS][2];
-    __shared__ float weight[AE_HEADS][16];
+    __shared__ float2 weight[AE_HEADS][16];
     const int tid = threadIdx.x, C = a.cluster, rank = blockIdx.x % C;
     for (int i = tid; i < heads * DIM; i += AE_THREADS) {
         float* at = red + i / DIM * S::RED + i % DIM;
@@ -233,17 +243,8 @@ __device__ __forceinline__ void share_row(const AttendE4& a, float* red, float (
         for (int w = 0; w < AE_WARPS; ++w) v += at[w * AE_HEADS * S::RED];
         *at = v;
     }
-    if (tid < AE_HEADS) {
-        float M = -INFINITY, L = 0.f;
-#pragma unroll
-        for (int w = 0; w < AE_WARPS; ++w) M = fmaxf(M, stat[w][tid][0]);
-#pragma unroll
-        for (int w = 0; w < AE_WARPS; ++w) L += stat[w][tid][1] * (M == -INFINITY ? 1.f : ex2(stat[w][tid][0] - M));
-        ml[tid][0] = M;
-        ml[tid][1] = L;
-    }
     cluster_meet();
-    // a thread a (head, CTA): what the CTA's sums are multiplied by
+    // a thread a (head, CTA): what the CTA's outputs are multiplied by
     static_assert(AE_THREADS == 16 * AE_HEADS, "16 CTAs at most for each of the heads");
     {
         const int h = tid >> 4, r = tid & 15;
@@ -257,19 +258,20 @@ __device__ __forceinline__ void share_row(const AttendE4& a, float* red, float (
         for (int o = 8; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
         const float sink = a.sinks && h < heads ? a.sinks[h0 + h] * 1.4426950408889634f : -INFINITY;
         M = fmaxf(M, sink);
-        const float w = M == -INFINITY ? 1.f : ex2(m - M);
-        float L = l * w;
+        if (M == -INFINITY) M = 0.f;
+        float L = l * ex2(m - M);
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-        if (sink != -INFINITY) L += ex2(sink - M);
-        weight[h][r] = L == 0.f ? 0.f : w / L;
+        L += ex2(sink - M);
+        const float2 f = two_factors(m - M, 0.f);
+        weight[h][r] = make_float2(f.x, L == 0.f ? 0.f : f.y * (l / L));
     }
     __syncthreads();
     T* out = (T*)a.out + ((size_t)b * a.nh + h0) * a.hdv;
     for (int i = rank * AE_THREADS + tid; i < heads * a.hdv; i += C * AE_THREADS) {
         const int h = i / a.hdv, d = i % a.hdv;
         float v = 0.f;
-        for (int r = 0; r < C; ++r) v += peer_f32(red + h * S::RED + d, r) * weight[h][r];
+        for (int r = 0; r < C; ++r) v += peer_f32(red + h * S::RED + d, r) * weight[h][r].x * weight[h][r].y;
         out[i] = from_f32<T>(v);
     }
     cluster_meet();                            // (a CTA's memory stays until its peers have read it)
@@ -284,7 +286,8 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
     constexpr int NQ = DIM / 64, NT = DIM / 16;
     constexpr int VB = DIM >= 128 ? 16 : 8, NV = DIM / (8 * VB); // bytes of values at a time, times
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ float stat[AE_WARPS][AE_HEADS][2];
+    // maxima and normalisers of the heads, each warp's and the CTA's
+    __shared__ __align__(16) float stat[AE_WARPS][AE_HEADS][2], ml[AE_HEADS][2];
     __shared__ float meta[AE_WARPS][S::STAGES][4];               // scales of keys and values, page is there
     pdl_wait();
     pdl_launch_next();
@@ -467,7 +470,8 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
             const float* bias1 = a.dist_bias ? a.dist_bias + (size_t)min(h0 + 2 * c + 1, a.nh - 1) * a.n_dist : nullptr;
 
             float o[NT][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-            float vref = AE_LEAST_SCALE, to_half = 16384.f / AE_LEAST_SCALE;
+            // the sums' references: e^u0 2^e0, e^u1 2^e1; the maxima above u0, u1
+            float u0 = -INFINITY, u1 = -INFINITY, e0 = 0.f, e1 = 0.f, g0 = 0.f, g1 = 0.f;
 #pragma unroll
             for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
 
@@ -516,14 +520,18 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
                 const unsigned char* V = mine + stage * S::STAGE + 16 * S::KS;
                 const bool there = meta[warp][stage][2] != 0.f;
                 const float ks = meta[warp][stage][0], vs = there ? meta[warp][stage][1] : 0.f;
-                const float g0 = ks * f0, g1 = ks * f1;
+                // the values' scale as vf 2^ve (vf is 1 for a power of two), 2^14 with it
+                const unsigned vb = min(__float_as_uint(vs) >> 23 & 0xffu, 253u);
+                const float ve = __uint_as_float(0x4b000000u | vb) - 8388735.f;      // (2^23 + vb) - 2^23 - 127
+                const float vf = vs * __uint_as_float((254u - vb) << 23) * 16384.f;
+                const float s0 = ks * f0, s1 = ks * f1;
                 // scores of positions j0 + r, j0 + r + 8 in units of ln 2
                 const int ja = j0 + r, jb = ja + 8;
                 const bool see_a = there && ja <= s.p && (ja >= s.first || ja < s.kept);
                 const bool see_b = there && jb <= s.p && (jb >= s.first || jb < s.kept);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    p[e] *= e & 1 ? g1 : g0;
+                    p[e] *= e & 1 ? s1 : s0;
                     if (EXTRAS) {
                         if (a.softcap > 0.f) p[e] = soft_capped_ex2(p[e], cap_unit, a.softcap);
                         if (a.dist_bias) p[e] += (e & 1 ? bias1 : bias)[min(max(s.p - (e >> 1 ? jb : ja), 0), a.n_dist - 1)];
@@ -537,25 +545,30 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
                     t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, w));
                     t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, w));
                 }
-                t0 = fmaxf(t0, m0);
-                t1 = fmaxf(t1, m1);
-                const float u0 = t0 == -INFINITY ? 0.f : t0, u1 = t1 == -INFINITY ? 0.f : t1;
-                float k0 = ex2(m0 - u0), k1 = ex2(m1 - u1);
-                m0 = t0;
-                m1 = t1;
-                p[0] = ex2(p[0] - u0);
-                p[1] = ex2(p[1] - u1);
-                p[2] = ex2(p[2] - u0);
-                p[3] = ex2(p[3] - u1);
-                l0 = fmaf(l0, k0, p[0] + p[2]);
-                l1 = fmaf(l1, k1, p[1] + p[3]);
-                // a greater maximum, or a greater scale of values than any before
-                if (__any_sync(0xffffffffu, k0 != 1.f || k1 != 1.f || vs > vref)) {
-                    if (vs > vref) {
-                        k0 *= vref / vs;
-                        k1 *= vref / vs;
-                        vref = vs;
-                        to_half = 16384.f / vref;
+                // A greater maximum, a greater product of a weight and its scale than any before (neither is so where
+                // no key is seen), or a scale so far above the reference's that products matter where the
+                // weights, as 32-bit numbers, are 0?
+                const float d0 = ve - e0, d1 = ve - e1, x0 = g0 + d0, x1 = g1 + d1;
+                const float up0 = (t0 - u0) + d0, up1 = (t1 - u1) + d1;
+                if (__any_sync(0xffffffffu, t0 > m0 || t1 > m1 || up0 > 0.f || up1 > 0.f || fmaxf(x0, x1) > 60.f)) {
+                    if (t0 > m0) {
+                        l0 *= ex2(m0 - t0);
+                        m0 = t0;
+                    }
+                    if (t1 > m1) {
+                        l1 *= ex2(m1 - t1);
+                        m1 = t1;
+                    }
+                    float k0 = 1.f, k1 = 1.f;
+                    if (up0 > 0.f) {
+                        k0 = ex2(-up0);
+                        u0 = t0;
+                        e0 = ve;
+                    }
+                    if (up1 > 0.f) {
+                        k1 = ex2(-up1);
+                        u1 = t1;
+                        e1 = ve;
                     }
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
@@ -564,17 +577,32 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
                         o[t][2] *= k0;
                         o[t][3] *= k1;
                     }
-                }
-                const float vf = vs * to_half;
+                    const float n0 = m0 == -INFINITY ? 0.f : m0, n1 = m1 == -INFINITY ? 0.f : m1;
+                    const float w0 = u0 == -INFINITY ? 0.f : u0, w1 = u1 == -INFINITY ? 0.f : u1;
+                    g0 = n0 - w0;
+                    g1 = n1 - w1;
+                    l0 += ex2(p[0] - n0) + ex2(p[2] - n0);
+                    l1 += ex2(p[1] - n1) + ex2(p[3] - n1);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) p[e] *= vf;
+                    for (int e = 0; e < 4; ++e)
+                        p[e] = ex2((p[e] - (e & 1 ? w1 : w0)) + (ve - (e & 1 ? e1 : e0))) * vf;
+                } else {
+                    const float n0 = m0 == -INFINITY ? 0.f : m0, n1 = m1 == -INFINITY ? 0.f : m1;
+                    const float k0 = ex2(x0) * vf, k1 = ex2(x1) * vf;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) p[e] = ex2(p[e] - (e & 1 ? n1 : n0));
+                    l0 += p[0] + p[2];
+                    l1 += p[1] + p[3];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) p[e] *= e & 1 ? k1 : k0;
+                }
                 const unsigned h0w = half2_of(p[0], p[1]), h1w = half2_of(p[2], p[3]);
                 const unsigned b0 = transposed(h0w), b1 = transposed(h1w);
                 unsigned c0 = 0, c1 = 0;
                 if (SPLIT) {
-                    const float2 w0 = float2_of(h0w), w1 = float2_of(h1w);
-                    c0 = transposed(half2_of(p[0] - w0.x, p[1] - w0.y));
-                    c1 = transposed(half2_of(p[2] - w1.x, p[3] - w1.y));
+                    const float2 x0 = float2_of(h0w), x1 = float2_of(h1w);
+                    c0 = transposed(half2_of(p[0] - x0.x, p[1] - x0.y));
+                    c1 = transposed(half2_of(p[2] - x1.x, p[3] - x1.y));
                 }
                 // values: dimensions q * 8 VB + r * VB .. of positions 2 c, 2 c + 1, 2 c + 8, 2 c + 9
 #pragma unroll
@@ -622,22 +650,41 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
                 l0 += __shfl_xor_sync(0xffffffffu, l0, w);
                 l1 += __shfl_xor_sync(0xffffffffu, l1, w);
             }
-            if (r == 0) {
-                stat[warp][2 * c][0] = m0;
-                stat[warp][2 * c][1] = l0;
-                stat[warp][2 * c + 1][0] = m1;
-                stat[warp][2 * c + 1][1] = l1;
-            }
+            if (r == 0) *reinterpret_cast<float4*>(stat[warp][2 * c]) = make_float4(m0, l0, m1, l1);
             __syncthreads();
-            float M0 = -INFINITY, M1 = -INFINITY;
+            // the CTA's, with the sink where this is all of the row
+            float M0 = -INFINITY, M1 = -INFINITY, L0, L1;
+            {
+                float4 of[AE_WARPS];
 #pragma unroll
-            for (int w = 0; w < AE_WARPS; ++w) {
-                M0 = fmaxf(M0, stat[w][2 * c][0]);
-                M1 = fmaxf(M1, stat[w][2 * c + 1][0]);
+                for (int w = 0; w < AE_WARPS; ++w) {
+                    of[w] = *reinterpret_cast<const float4*>(stat[w][2 * c]);
+                    M0 = fmaxf(M0, of[w].x);
+                    M1 = fmaxf(M1, of[w].z);
+                }
+                float sink0 = -INFINITY, sink1 = -INFINITY;
+                if (a.sinks && whole && !shared_row) {
+                    if (2 * c < heads) sink0 = a.sinks[h0 + 2 * c] * LOG2E;
+                    if (2 * c + 1 < heads) sink1 = a.sinks[h0 + 2 * c + 1] * LOG2E;
+                    M0 = fmaxf(M0, sink0);
+                    M1 = fmaxf(M1, sink1);
+                }
+                const float n0 = M0 == -INFINITY ? 0.f : M0, n1 = M1 == -INFINITY ? 0.f : M1;
+                L0 = ex2(sink0 - n0);
+                L1 = ex2(sink1 - n1);
+#pragma unroll
+                for (int w = 0; w < AE_WARPS; ++w) {
+                    L0 = fmaf(of[w].y, ex2(of[w].x - n0), L0);
+                    L1 = fmaf(of[w].w, ex2(of[w].z - n1), L1);
+                }
+                if (tid < 4) *reinterpret_cast<float4*>(ml[2 * c]) = make_float4(M0, L0, M1, L1);
+                M0 = n0;
+                M1 = n1;
             }
-            const float back = vref * (1.f / 16384.f);
-            const float k0 = (M0 == -INFINITY ? 1.f : ex2(m0 - M0)) * back;
-            const float k1 = (M1 == -INFINITY ? 1.f : ex2(m1 - M1)) * back;
+            // what brings this warp's sums to outputs: 2^-14 e^(u - maximum) 2^e / normaliser
+            float2 k0 = two_factors(u0 - M0, e0), k1 = two_factors(u1 - M1, e1);
+            k0.y *= L0 == 0.f ? 0.f : __fdividef(1.f / 16384.f, L0);
+            k1.y *= L1 == 0.f ? 0.f : __fdividef(1.f / 16384.f, L1);
             float* red = reinterpret_cast<float*>(smem);
 #pragma unroll
             for (int q = 0; q < NV; ++q) {
@@ -647,45 +694,32 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
                 for (int e = 0; e < VB / 4; ++e) {
                     const int t = q * (VB / 2) + 2 * e;
                     *reinterpret_cast<float4*>(d0 + 4 * e) =
-                        make_float4(o[t][0] * k0, o[t][2] * k0, o[t + 1][0] * k0, o[t + 1][2] * k0);
+                        make_float4(o[t][0] * k0.y * k0.x, o[t][2] * k0.y * k0.x, o[t + 1][0] * k0.y * k0.x,
+                                    o[t + 1][2] * k0.y * k0.x);
                     *reinterpret_cast<float4*>(d1 + 4 * e) =
-                        make_float4(o[t][1] * k1, o[t][3] * k1, o[t + 1][1] * k1, o[t + 1][3] * k1);
+                        make_float4(o[t][1] * k1.y * k1.x, o[t][3] * k1.y * k1.x, o[t + 1][1] * k1.y * k1.x,
+                                    o[t + 1][3] * k1.y * k1.x);
                 }
             }
             __syncthreads();
             float* part = nullptr;
             if (a.partial) part = a.partial + gridDim.x / R * 4 + (size_t)(2 * blockIdx.x + (segment > 0)) * S::PART;
             if (shared_row) {
-                share_row<T, DIM>(a, red, stat, b, h0, heads);
+                share_row<T, DIM>(a, red, ml, b, h0, heads);
                 return;
             }
             for (int i = tid; i < heads * DIM; i += AE_THREADS) {
                 const int h = i / DIM, d = i % DIM;
                 if (d >= a.hdv) continue;
-                float v = 0.f, L = 0.f, M = -INFINITY;
+                float v = 0.f;
 #pragma unroll
-                for (int w = 0; w < AE_WARPS; ++w) {
-                    v += red[(w * AE_HEADS + h) * S::RED + d];
-                    M = fmaxf(M, stat[w][h][0]);
-                }
-#pragma unroll
-                for (int w = 0; w < AE_WARPS; ++w)
-                    L += stat[w][h][1] * (stat[w][h][0] == M || M == -INFINITY ? 1.f : ex2(stat[w][h][0] - M));
-                if (!whole) {
-                    part[h * DIM + d] = v;
-                    if (d == 0) {
-                        part[AE_HEADS * DIM + 2 * h] = M;
-                        part[AE_HEADS * DIM + 2 * h + 1] = L;
-                    }
+                for (int w = 0; w < AE_WARPS; ++w) v += red[(w * AE_HEADS + h) * S::RED + d];
+                if (whole) {
+                    ((T*)a.out)[((size_t)b * a.nh + h0 + h) * a.hdv + d] = from_f32<T>(v);
                     continue;
                 }
-                if (a.sinks) {
-                    const float sink = a.sinks[h0 + h] * LOG2E, N = fmaxf(M, sink);
-                    const float f = M == -INFINITY ? 0.f : ex2(M - N);
-                    L = L * f + ex2(sink - N);
-                    v *= f;
-                }
-                ((T*)a.out)[((size_t)b * a.nh + h0 + h) * a.hdv + d] = from_f32<T>(L == 0.f ? 0.f : v / L);
+                part[h * DIM + d] = v;
+                if (d < 2) part[AE_HEADS * DIM + 2 * h + d] = ml[h][d];
             }
             __syncthreads();
         }
@@ -706,7 +740,7 @@ constexpr int AE_MAX_STRETCHES = 1024;
 template <typename T, int DIM>
 __global__ void __launch_bounds__(AE_JOIN_THREADS) join_e4m3_kernel(const AttendE4 a, int stretches) {
     using S = Tile<DIM>;
-    __shared__ float weight[AE_MAX_STRETCHES];
+    __shared__ float2 weight[AE_MAX_STRETCHES];
     __shared__ int slot[AE_MAX_STRETCHES];
     __shared__ float scratch[32];
     __shared__ float4 sums[AE_JOIN_THREADS];
@@ -729,20 +763,23 @@ __global__ void __launch_bounds__(AE_JOIN_THREADS) join_e4m3_kernel(const Attend
             const int part = i - 1 + j, from = stretch_start(total, part, stretches);
             const int at = from == stretch_start(total, part + 1, stretches) ? -1 : 2 * (part * R + row) + (from < begin);
             slot[j] = at;
-            weight[j] = at < 0 ? -INFINITY : partial[(size_t)at * S::PART + AE_HEADS * DIM + 2 * head];
-            M = fmaxf(M, weight[j]);
+            weight[j] = at < 0 ? make_float2(-INFINITY, 0.f) : *reinterpret_cast<const float2*>(
+                                     partial + (size_t)at * S::PART + AE_HEADS * DIM + 2 * head);
+            M = fmaxf(M, weight[j].x);
         }
         M = block_max(M, scratch);
         const float sink = a.sinks ? a.sinks[h0 + head] * 1.4426950408889634f : -INFINITY;
         M = fmaxf(M, sink);
+        if (M == -INFINITY) M = 0.f;
         float L = 0.f;
         for (int j = tid; j < parts; j += AE_JOIN_THREADS) {
-            const float w = M == -INFINITY ? 1.f : ex2(weight[j] - M);
-            weight[j] = w;
-            if (slot[j] >= 0) L += w * partial[(size_t)slot[j] * S::PART + AE_HEADS * DIM + 2 * head + 1];
+            const float2 ml = weight[j], f = two_factors(ml.x - M, 0.f);
+            L = fmaf(ml.y, ex2(ml.x - M), L);
+            weight[j] = make_float2(f.x, f.y * ml.y);
         }
         L = block_sum(L, scratch);                 // (with barriers: the weights are there)
-        if (sink != -INFINITY) L += ex2(sink - M);
+        L += ex2(sink - M);
+        const float inverse = L == 0.f ? 0.f : 1.f / L;
         constexpr int LANES = DIM / 4, GROUPS = AE_JOIN_THREADS / LANES;
         const int d = tid % LANES * 4;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -752,11 +789,11 @@ __global__ void __launch_bounds__(AE_JOIN_THREADS) join_e4m3_kernel(const Attend
                 const int at = slot[j];
                 if (at < 0) continue;
                 const float4 u = *reinterpret_cast<const float4*>(partial + (size_t)at * S::PART + head * DIM + d);
-                const float w = weight[j];
-                v.x = fmaf(u.x, w, v.x);
-                v.y = fmaf(u.y, w, v.y);
-                v.z = fmaf(u.z, w, v.z);
-                v.w = fmaf(u.w, w, v.w);
+                const float f = weight[j].x, w = weight[j].y * inverse;
+                v.x = fmaf(u.x * f, w, v.x);
+                v.y = fmaf(u.y * f, w, v.y);
+                v.z = fmaf(u.z * f, w, v.z);
+                v.w = fmaf(u.w * f, w, v.w);
             }
         }
         sums[tid] = v;
@@ -767,7 +804,7 @@ __global__ void __launch_bounds__(AE_JOIN_THREADS) join_e4m3_kernel(const Attend
             float o = 0.f;
 #pragma unroll
             for (int q = 0; q < GROUPS; ++q) o += flat[q * DIM + e];
-            out[e] = from_f32<T>(L == 0.f ? 0.f : o / L);
+            out[e] = from_f32<T>(o);
         }
     }
 }

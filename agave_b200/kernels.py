@@ -2164,8 +2164,10 @@ def attention_decode_e4m3(q: torch.Tensor, out: torch.Tensor, view, ctx, n_heads
                           softcap: float = 0.0, op: str = "attention") -> None:
     """Decode attention of one layer over a cache entry that holds e4m3 codes
     (``cache_store_e4m3``): q [B, nh * hd] (rows may be strided) at ``ctx.positions``, out
-    [B, nh * hdv] of the same type.  Codes are exact in the products; sums, the softmax and its
-    weights are 32-bit (of bfloat16 queries the weights are rounded to 11 bits).  Options as in
+    [B, nh * hdv] of the same type.  Codes are exact in the products; sums and the softmax are
+    32-bit.  Pages may have scales anywhere in 2^-126 .. 2^120, whichever way they lie: a weight times
+    its page's scale is off by at most 2^-22 of itself (2^-11 for bfloat16 queries) or 2^-39 of the row's
+    greatest such product in the product with the values.  Options as in
     ``attention_decode``; rows of entries with a negative slot become zeros.  ``ctx.max_len``
     bounds the lengths (it sizes the grid and the scratch; a longer sequence is still walked
     whole)."""
