@@ -293,11 +293,12 @@ class Engine:
             raise
 
     def cancel(self) -> None:
-        """Stop the running ``generate`` or ``step`` at its next check, from any thread
+        """Stop the running ``generate``, ``score`` or ``step`` at its next check, from any thread
         (src/models/model.zig:443-446).  A step that runs launch by launch stops between
         two blocks (src/models/gemma3.zig:342,435); a recorded step runs to its end, and
         the generation loop stops before the next one.  ``generate`` then returns what
-        was generated so far, with the finish reason "cancelled" for what it cut."""
+        was generated so far, with the finish reason "cancelled" for what it cut; ``score`` looks
+        between blocks and between portions of logits, and raises ``Cancelled``."""
         self._cancel.set()
 
     # ------------------------------------------------------------- generate
@@ -348,7 +349,8 @@ class Engine:
         it: one ``TokenScore`` each (their sum of log-probabilities is the sequence's).
 
         Sequences run whole, as prompts do, as many at a time as the cache holds; the logits of
-        some rows at a time are formed and read, so no whole [tokens, vocabulary] is held."""
+        some rows at a time are formed and read, so no whole [tokens, vocabulary] is held.
+        Raises ``Cancelled`` when ``cancel()`` was called before its last portion of them."""
         if not 0 <= top <= min(kernels.LOGPROBS_MAX_TOP, self.spec.vocab_size):
             raise ValueError(f"top must lie in 0..{kernels.LOGPROBS_MAX_TOP}")
         plan = GenerationPlan(sequences, 1, (), self.max_batch, self.max_tokens, self.max_seq_len)
@@ -360,9 +362,8 @@ class Engine:
                     return out
                 self._score_batch(batch, top, out)
                 plan.accept({r.index: 0 for r in batch})
-        except Cancelled:
+        finally:
             self._cancel.clear()
-            raise
 
     def _score_batch(self, batch, top: int, out: List[List[TokenScore]]) -> None:
         for r in batch:
@@ -383,6 +384,8 @@ class Engine:
             packed = torch.empty(kernels.token_logprobs_words(min(step, len(rows)), top),
                                  dtype=torch.float32, device=self.device)
             for a in range(0, len(rows), step):
+                if self._cancel.is_set():
+                    raise Cancelled("cancelled between two portions of logits")
                 logits = self.model.logits(h, both[0, a:a + step], ctx)
                 n = logits.shape[0]
                 kernels.token_logprobs(logits, both[1, a:a + step], top, packed=packed)
