@@ -35,6 +35,7 @@
 // takes nothing but the maxima and normalisers.
 #include "e4m3.cuh"
 #include <atomic>
+#include <cfloat>
 
 namespace {
 
@@ -535,7 +536,10 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
                     if (EXTRAS) {
                         if (a.softcap > 0.f) p[e] = soft_capped_ex2(p[e], cap_unit, a.softcap);
                         if (a.dist_bias) p[e] += (e & 1 ? bias1 : bias)[min(max(s.p - (e >> 1 ? jb : ja), 0), a.n_dist - 1)];
-                        p[e] *= LOG2E;
+                        // (a finite score stays finite: a bias of the type's lowest value is no -inf, and
+                        // where every key has it they weigh the same)
+                        const float x = p[e] * LOG2E;
+                        p[e] = x == -INFINITY && p[e] != -INFINITY ? -FLT_MAX : x;
                     }
                     if (!(e >> 1 ? see_b : see_a)) p[e] = -INFINITY;
                 }

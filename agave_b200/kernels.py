@@ -2168,7 +2168,8 @@ def attention_decode_e4m3(q: torch.Tensor, out: torch.Tensor, view, ctx, n_heads
     32-bit.  Pages may have scales anywhere in 2^-126 .. 2^120, whichever way they lie: a weight times
     its page's scale is off by at most 2^-22 of itself (2^-11 for bfloat16 queries) or 2^-39 of the row's
     greatest such product in the product with the values.  Options as in
-    ``attention_decode``; rows of entries with a negative slot become zeros.  ``ctx.max_len``
+    ``attention_decode``; a bias of -inf hides its key; rows of entries with a negative slot, and heads that
+    see no key, become zeros.  ``ctx.max_len``
     bounds the lengths (it sizes the grid and the scratch; a longer sequence is still walked
     whole)."""
     hdv = value_dim or head_dim
