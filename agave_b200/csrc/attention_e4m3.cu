@@ -818,16 +818,18 @@ struct Plan {
     bool split;                // stretches of an equal number of tiles, joined afterwards
     int stretches;             // so many for each row
     int cluster;               // else: CTAs that share a row
+    int sms;                   // of the device
 };
+// Of the current device, asked once for each (148 where there is none to ask, as in a plan made on the host).
 int sm_count() {
-    static int n = 0;
-    if (n == 0) {
-        int dev = 0, v = 0;
-        if (cudaGetDevice(&dev) == cudaSuccess &&
-            cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess)
-            n = v;
-    }
-    return n > 0 ? n : 148;
+    static std::atomic<int> counts[64];
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+    std::atomic<int>& known = counts[dev & 63];          // (of devices from 64 on nothing is kept)
+    if (dev < 64 && (n = known.load()) > 0) return n;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) return 148;
+    if (dev < 64) known.store(n);
+    return n;
 }
 Plan plan_of(int B, int nh, int nkv, int hd, int hdv, int max_keys) {
     Plan p;
@@ -836,7 +838,8 @@ Plan plan_of(int B, int nh, int nkv, int hd, int hdv, int max_keys) {
     const int R = nkv * ((nh / nkv + AE_HEADS - 1) / AE_HEADS);
     const long long rows = (long long)B * R;
     const long long tiles = ((long long)max_keys + AE_TILE - 1) / AE_TILE + 1;
-    const int resident = sm_count() * (p.dim == 256 ? Tile<256>::CTAS : p.dim == 128 ? Tile<128>::CTAS : Tile<64>::CTAS);
+    p.sms = sm_count();
+    const int resident = p.sms * (p.dim == 256 ? Tile<256>::CTAS : p.dim == 128 ? Tile<128>::CTAS : Tile<64>::CTAS);
     // A row is the work of a cluster where that leaves each of its CTAs a few tiles: one launch, and the
     // join goes through shared memory.  As many CTAs as run at a time, 16 only where those are few
     // (one row of 2000 keys: 32 us with one, 14 with four, 11 with eight, 9.7 with 16; 32 rows of 1000: 19, 12, 11, 26).
@@ -844,7 +847,7 @@ Plan plan_of(int B, int nh, int nkv, int hd, int hdv, int max_keys) {
     // 11 with 16 CTAs a row, of 16000: 21 and 23; 256 rows of 1500: 40 and 36 with one CTA a row, of
     // 4000: 62 and 75).
     p.cluster = 1;
-    while (p.cluster < 16 && p.cluster < tiles && rows * p.cluster * 2 <= (p.cluster < 8 ? resident : sm_count()))
+    while (p.cluster < 16 && p.cluster < tiles && rows * p.cluster * 2 <= (p.cluster < 8 ? resident : p.sms))
         p.cluster *= 2;
     p.split = tiles > (p.cluster < 8 ? 40 * p.cluster : 240);
     long long stretches = resident / R;                          // all CTAs at a time
@@ -870,7 +873,7 @@ int launch(const AttendE4& a, const Plan& p, cudaStream_t stream) {
     if (p.stretches > 1) {
         // (a CTA a head while that makes no more CTAs than run at a time)
         const int R = a.nkv * a.row_blocks, heads = a.nh / a.nkv < AE_HEADS ? a.nh / a.nkv : AE_HEADS;
-        const int y = 4 * sm_count() / ((p.stretches - 1) * R);
+        const int y = 4 * p.sms / ((p.stretches - 1) * R);
         agv_launch(join_e4m3_kernel<T, DIM>, dim3(p.stretches - 1, y < 1 ? 1 : y < heads ? y : heads, R), AE_JOIN_THREADS, 0,
                    stream, a, p.stretches);
         AGV_LAUNCH_OK("join_e4m3_kernel");
