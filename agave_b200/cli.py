@@ -245,6 +245,18 @@ def _score_record(s) -> dict:
             "rank": s.rank, "top": [[i, _number(lp)] for i, lp in s.top]}
 
 
+def _perplexity(scores) -> Optional[float]:
+    """e^-(mean log-probability); None where nothing was scored, where a token has no finite
+    log-probability and where the number would leave the range of floats."""
+    if not scores:
+        return None
+    mean = sum(s.logprob for s in scores) / len(scores)
+    try:
+        return _number(math.exp(-mean))
+    except OverflowError:
+        return None
+
+
 def _score_prompts(engine, prompts, args) -> int:
     """``--score``: what the model gives the prompts' own tokens."""
     try:
@@ -253,10 +265,8 @@ def _score_prompts(engine, prompts, args) -> int:
         return _fail(str(e))
     recs = []
     for p, row in zip(prompts, scores):
-        total = sum(s.logprob for s in row)
-        mean = total / len(row) if row else 0.0
-        recs.append({"tokens": len(p), "logprob_sum": _number(total),
-                     "perplexity": _number(math.exp(min(-mean, 700.0))),
+        recs.append({"tokens": len(p), "logprob_sum": _number(sum(s.logprob for s in row)),
+                     "perplexity": _perplexity(row),
                      "logprobs": [_score_record(s) for s in row]})
     if args.json:
         print(json.dumps(recs[0] if len(recs) == 1 else recs))
@@ -265,7 +275,8 @@ def _score_prompts(engine, prompts, args) -> int:
         for s in row:
             print(f"{s.token}\t{s.logprob:.6f}\t{s.rank}")
         if not args.quiet:
-            print(f"{rec['tokens']} tok · perplexity {rec['perplexity']}", file=sys.stderr)
+            perplexity = "none" if rec["perplexity"] is None else rec["perplexity"]
+            print(f"{rec['tokens']} tok · perplexity {perplexity}", file=sys.stderr)
     return 0
 
 

@@ -1,0 +1,42 @@
+"""What ``--score`` and ``--logprobs`` print, with an engine that answers by rote."""
+import json
+import math
+from types import SimpleNamespace
+
+import pytest
+
+from agave_b200.sampling import TokenScore
+
+
+def printed(capsys, logprobs, json_out=True, prompt=None):
+    from agave_b200.cli import _score_prompts
+    row = [TokenScore(i, lp, 1.0, 1) for i, lp in enumerate(logprobs)]
+    engine = SimpleNamespace(score=lambda prompts, top: [row])
+    args = SimpleNamespace(logprobs=None, json=json_out, quiet=False)
+    assert _score_prompts(engine, [prompt or [1] * (len(row) + 1)], args) == 0
+    return capsys.readouterr()
+
+
+def strict(text):
+    def refuse(name):
+        raise ValueError(name)
+    return json.loads(text, parse_constant=refuse)
+
+
+@pytest.mark.parametrize("logprobs,total,perplexity", [
+    ([], 0, None),                                            # one token: nothing scored
+    ([-1.0, -3.0], -4.0, math.exp(2.0)),
+    ([0.0], 0.0, 1.0),
+    ([-1.0, -math.inf], None, None),                          # an impossible token
+    ([math.nan, -1.0], None, None),
+    ([-2000.0, -1000.0], -3000.0, None),                      # e^1500 is no float
+    ([-700.0], -700.0, math.exp(700.0)),
+])
+def test_perplexity(capsys, logprobs, total, perplexity):
+    rec = strict(printed(capsys, logprobs).out)
+    assert rec["logprob_sum"] == total
+    assert rec["perplexity"] is None if perplexity is None else abs(rec["perplexity"] / perplexity - 1) < 1e-12
+    assert [r["logprob"] for r in rec["logprobs"]] == [lp if math.isfinite(lp) else None for lp in logprobs]
+    text = printed(capsys, logprobs, json_out=False)
+    assert len(text.out.splitlines()) == len(logprobs)
+    assert text.err.strip().endswith("none" if perplexity is None else str(rec["perplexity"]))
