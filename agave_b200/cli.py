@@ -260,7 +260,7 @@ def _perplexity(scores) -> Optional[float]:
 def _score_prompts(engine, prompts, args) -> int:
     """``--score``: what the model gives the prompts' own tokens."""
     try:
-        scores = engine.score(prompts, top=args.logprobs or 0)
+        scores = engine.score(prompts, top=(args.logprobs or 0) if args.json else 0)
     except (ValueError, RuntimeError) as e:
         return _fail(str(e))
     recs = []
@@ -417,7 +417,8 @@ def main(argv: Optional[List[str]] = None) -> int:
         outs = engine.generate(prompts, max_new_tokens=args.max_tokens,
                                temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
                                repeat_penalty=args.repeat_penalty, seed=args.seed,
-                               stop_token_ids=stops, logprobs=args.logprobs)
+                               stop_token_ids=stops,
+                               logprobs=args.logprobs if args.json else None)      # (only there printed)
     except (ValueError, RuntimeError) as e:
         return _fail(str(e))
     finally:

@@ -40,3 +40,35 @@ def test_perplexity(capsys, logprobs, total, perplexity):
     text = printed(capsys, logprobs, json_out=False)
     assert len(text.out.splitlines()) == len(logprobs)
     assert text.err.strip().endswith("none" if perplexity is None else str(rec["perplexity"]))
+
+
+@pytest.mark.parametrize("json_out", [True, False])
+@pytest.mark.parametrize("score", [True, False])
+def test_log_probabilities_are_asked_for_where_they_are_printed(tmp_path, monkeypatch, capsys, json_out, score):
+    from agave_b200 import cli
+    from agave_b200.engine import api
+    from util import TINY
+    asked = []
+
+    class Recorder:
+        max_seq_len, load_seconds, ignored_tensors = 64, 0.0, ()
+
+        @classmethod
+        def from_config(cls, *args, **kw):
+            return cls()
+
+        def model_info(self):
+            return {"config": {}, "dtype": "bfloat16", "weight_bytes": 0, "cache_bytes": 0}
+
+        def generate(self, prompts, logprobs=None, **kw):
+            asked.append(logprobs)
+            raise RuntimeError("asked")
+
+        def score(self, prompts, top=0):
+            asked.append(top)
+            raise RuntimeError("asked")
+    monkeypatch.setattr(api, "Engine", Recorder)
+    (tmp_path / "config.json").write_text(json.dumps(TINY["A"][0]))
+    argv = [str(tmp_path), "--random-weights", "1", "--tokens", "1,2", "--logprobs", "4"]
+    assert cli.main(argv + ["--json"] * json_out + ["--score"] * score) == 1
+    assert asked == [4 if json_out else 0 if score else None]
