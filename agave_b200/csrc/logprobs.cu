@@ -500,12 +500,15 @@ int lp_cluster_bits(int R, int V) {
     return bits;
 }
 
-// Threads of a CTA: 512 for few or long rows, else fewer, so that the rows run at a time (an SM takes
-// 1024 threads) and what a CTA does besides reading runs under the others' reads (us with 128, 256 and
-// 512 threads: 300 rows of 32001 24, 17 and 20; 777 bfloat16 rows of 32001 26.5, 24.6 and 33, 1100 30, 32
-// and 42; 1000 rows of 5000 12, 15 and 21; 600 of 100000 78, 65 and 59).
+// Threads of a CTA.  An SM takes 1024: 512 a CTA where that holds all CTAs at a time (296), and for long rows; 256 up
+// to 592; above that the CTAs come in rounds, and what one does besides reading runs under the others' reads, of
+// which rows up to 32768 logits have most with 128 threads, longer ones with 256 (us with 128, 256 and 512
+// threads, five alternatives; 32-bit, then bfloat16: 300 rows of 32001 19, 15, 18 and 15, 15, 17; 777 of 9000 14, 16,
+// 20 and 14, 16, 19; of 16384 17, 20, 23 and 17, 19, 25; of 32001 29, 31, 32 and 26, 26, 31; of 48000 39, 41, 38 and
+// 34, 31, 36; 1500 of 16384 30, 31, 40 and 25, 29, 43; of 32001 50, 47, 53 and 38, 41, 54; of 65000 92, 80, 81 and
+// 58, 58, 70; 600 of 100000 in 32 bits 78, 65, 59).
 int lp_threads(long long ctas, int V) {
-    return ctas <= 296 || V > 65536 ? 512 : ctas <= (V > 8192 ? 1000 : 592) ? 256 : 128;
+    return ctas <= 296 || V > 65536 ? 512 : ctas <= 592 || V > 32768 ? 256 : 128;
 }
 
 template <typename T, bool TOP, int THREADS>
