@@ -265,13 +265,14 @@ __device__ __forceinline__ void share_row(const AttendE4& a, float* red, const f
         for (int o = 8; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
         L += ex2(sink - M);
         const float2 f = two_factors(m - M, 0.f);
-        weight[h][r] = make_float2(f.x, L == 0.f ? 0.f : f.y * (l / L));
+        weight[h][r] = make_float2(f.x, L == 0.f ? 0.f : f.y * __fdividef(l, L));
     }
     __syncthreads();
     T* out = (T*)a.out + ((size_t)b * a.nh + h0) * a.hdv;
     for (int i = rank * AE_THREADS + tid; i < heads * a.hdv; i += C * AE_THREADS) {
         const int h = i / a.hdv, d = i % a.hdv;
         float v = 0.f;
+#pragma unroll 4
         for (int r = 0; r < C; ++r) v += peer_f32(red + h * S::RED + d, r) * weight[h][r].x * weight[h][r].y;
         out[i] = from_f32<T>(v);
     }
@@ -552,8 +553,10 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
                 // A greater maximum, a greater product of a weight and its scale than any before (neither is so where
                 // no key is seen), or a scale so far above the reference's that products matter where the
                 // weights, as 32-bit numbers, are 0?
-                const float d0 = ve - e0, d1 = ve - e1, x0 = g0 + d0, x1 = g1 + d1;
+                const float d0 = ve - e0, d1 = ve - e1;
+                float x0 = g0 + d0, x1 = g1 + d1;
                 const float up0 = (t0 - u0) + d0, up1 = (t1 - u1) + d1;
+                bool far = false;
                 if (__any_sync(0xffffffffu, t0 > m0 || t1 > m1 || up0 > 0.f || up1 > 0.f || fmaxf(x0, x1) > 60.f)) {
                     if (t0 > m0) {
                         l0 *= ex2(m0 - t0);
@@ -574,6 +577,11 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
                         u1 = t1;
                         e1 = ve;
                     }
+                    g0 = m0 == u0 ? 0.f : m0 - u0;               // (both -inf: nothing seen yet)
+                    g1 = m1 == u1 ? 0.f : m1 - u1;
+                    x0 = g0 + (ve - e0);
+                    x1 = g1 + (ve - e1);
+                    far = __any_sync(0xffffffffu, fmaxf(x0, x1) > 60.f);
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
                         o[t][0] *= k0;
@@ -581,17 +589,9 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
                         o[t][2] *= k0;
                         o[t][3] *= k1;
                     }
-                    const float n0 = m0 == -INFINITY ? 0.f : m0, n1 = m1 == -INFINITY ? 0.f : m1;
-                    const float w0 = u0 == -INFINITY ? 0.f : u0, w1 = u1 == -INFINITY ? 0.f : u1;
-                    g0 = n0 - w0;
-                    g1 = n1 - w1;
-                    l0 += ex2(p[0] - n0) + ex2(p[2] - n0);
-                    l1 += ex2(p[1] - n1) + ex2(p[3] - n1);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        p[e] = ex2((p[e] - (e & 1 ? w1 : w0)) + (ve - (e & 1 ? e1 : e0))) * vf;
-                } else {
-                    const float n0 = m0 == -INFINITY ? 0.f : m0, n1 = m1 == -INFINITY ? 0.f : m1;
+                }
+                const float n0 = m0 == -INFINITY ? 0.f : m0, n1 = m1 == -INFINITY ? 0.f : m1;
+                if (!far) {
                     const float k0 = ex2(x0) * vf, k1 = ex2(x1) * vf;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) p[e] = ex2(p[e] - (e & 1 ? n1 : n0));
@@ -599,6 +599,13 @@ __global__ void __launch_bounds__(AE_THREADS, Tile<DIM>::CTAS) attend_e4m3_kerne
                     l1 += p[1] + p[3];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) p[e] *= e & 1 ? k1 : k0;
+                } else {
+                    const float w0 = u0 == -INFINITY ? 0.f : u0, w1 = u1 == -INFINITY ? 0.f : u1;
+                    l0 += ex2(p[0] - n0) + ex2(p[2] - n0);
+                    l1 += ex2(p[1] - n1) + ex2(p[3] - n1);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        p[e] = ex2((p[e] - (e & 1 ? w1 : w0)) + (ve - (e & 1 ? e1 : e0))) * vf;
                 }
                 const unsigned h0w = half2_of(p[0], p[1]), h1w = half2_of(p[2], p[3]);
                 const unsigned b0 = transposed(h0w), b1 = transposed(h1w);
