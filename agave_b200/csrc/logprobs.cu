@@ -502,13 +502,13 @@ int lp_cluster_bits(int R, int V) {
 
 // Threads of a CTA.  An SM takes 1024: 512 a CTA where that holds all CTAs at a time (296), and for long rows; 256 up
 // to 592; above that the CTAs come in rounds, and what one does besides reading runs under the others' reads, of
-// which rows up to 32768 logits have most with 128 threads, longer ones with 256 (us with 128, 256 and 512
+// which rows up to 28000 logits have most with 128 threads, longer ones with 256 (us with 128, 256 and 512
 // threads, five alternatives; 32-bit, then bfloat16: 300 rows of 32001 19, 15, 18 and 15, 15, 17; 777 of 9000 14, 16,
-// 20 and 14, 16, 19; of 16384 17, 20, 23 and 17, 19, 25; of 32001 29, 31, 32 and 26, 26, 31; of 48000 39, 41, 38 and
-// 34, 31, 36; 1500 of 16384 30, 31, 40 and 25, 29, 43; of 32001 50, 47, 53 and 38, 41, 54; of 65000 92, 80, 81 and
-// 58, 58, 70; 600 of 100000 in 32 bits 78, 65, 59).
+// 20 and 14, 16, 19; of 16384 17, 20, 23 and 17, 19, 25; of 24000 23, 24, 28 and 22, 23, 28; of 32001 29, 31, 32 and 26,
+// 25, 31; of 48000 39, 41, 38 and 34, 31, 36; 1500 of 16384 30, 31, 40 and 25, 29, 43; of 24000 39, 39, 48 and 32, 35, 47; of
+// 32001 50, 47, 53 and 38, 41, 54; of 65000 92, 80, 81 and 58, 58, 70; 600 of 100000 in 32 bits 78, 65, 59).
 int lp_threads(long long ctas, int V) {
-    return ctas <= 296 || V > 65536 ? 512 : ctas <= 592 || V > 32768 ? 256 : 128;
+    return ctas <= 296 || V > 65536 ? 512 : ctas <= 592 || V > 28000 ? 256 : 128;
 }
 
 template <typename T, bool TOP, int THREADS>
