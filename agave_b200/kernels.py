@@ -2165,7 +2165,8 @@ def attention_decode_e4m3(q: torch.Tensor, out: torch.Tensor, view, ctx, n_heads
     """Decode attention of one layer over a cache entry that holds e4m3 codes
     (``cache_store_e4m3``): q [B, nh * hd] (rows may be strided) at ``ctx.positions``, out
     [B, nh * hdv] of the same type.  Codes are exact in the products; sums and the softmax are
-    32-bit.  Pages may have scales anywhere in 2^-126 .. 2^120, whichever way they lie: a weight times
+    32-bit; an element of a query is off by at most 2^-22 of itself (bfloat16: not at all) or 2^-34 of the
+    greatest of its head.  Pages may have scales anywhere in 2^-126 .. 2^120, whichever way they lie: a weight times
     its page's scale is off by at most 2^-22 of itself (2^-11 for bfloat16 queries) or 2^-39 of the row's
     greatest such product in the product with the values.  Options as in
     ``attention_decode``; a bias of -inf hides its key; rows of entries with a negative slot, and heads that
@@ -2210,7 +2211,7 @@ def attention_decode_e4m3(q: torch.Tensor, out: torch.Tensor, view, ctx, n_heads
     if dist_bias is not None:
         _on_current_device(dist_bias); _f32(dist_bias, "dist_bias")
         _require(dist_bias.dim() == 2 and dist_bias.shape[0] == n_heads and
-                 dist_bias.is_contiguous(),
+                 dist_bias.shape[1] > 0 and dist_bias.is_contiguous(),
                  "attention_decode_e4m3: the bias by distance is [heads, distances]")
         bias_at, n_dist = dist_bias.data_ptr(), dist_bias.shape[1]
     max_keys = max(1, min(abs(window) + keep_first, ctx.max_len) if window else ctx.max_len)

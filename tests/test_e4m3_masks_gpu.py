@@ -93,3 +93,13 @@ def test_the_same_call_gives_the_same_bits():
                 kernels.attention_decode_e4m3(q, out, view, ctx, nh, nkv, hd, 0.5 * hd ** -0.5, 0)
                 first = out if first is None else first
                 assert torch.equal(first, out)
+
+
+def test_a_bias_of_no_distances_is_refused():
+    """It has no address: taken as none, it would be left out without a word."""
+    from agave_b200 import kernels
+    view, q, ctx, nh, nkv, hd = setup(F32, 1)
+    for shape in ((nh, 0), (nh + 1, 3), (3,)):
+        with pytest.raises(kernels.KernelError, match="bias by distance"):
+            kernels.attention_decode_e4m3(q, torch.empty_like(q), view, ctx, nh, nkv, hd, 1.0, 0,
+                                          dist_bias=torch.zeros(shape, device=DEV))
