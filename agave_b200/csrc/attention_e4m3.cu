@@ -24,7 +24,8 @@
 // The next tile's products stand beside a tile's softmax and fill its waits (247 us, 238 with).
 //
 // Precision: codes are exact in half; a query is scaled by a power of two and split into two
-// halves (22 bits) where it is 32-bit; a bfloat16 one fits in one.  Weights are 32-bit, split the same
+// halves (22 bits) where it is 32-bit; a bfloat16 one fits in one (elements below 2^-26 of a head's
+// greatest keep fewer bits: they are off by up to 2^-34 of it).  Weights are 32-bit, split the same
 // way for 32-bit queries and rounded to 11 bits for bfloat16 ones, whose results keep 8.  The scale 2^e
 // of a page's values is part of the weights that are multiplied with them: the products e^s 2^e have
 // a reference of their own, the greatest so far, apart from the maximum of the scores, which the

@@ -2,9 +2,11 @@
 //
 // value = code * scale.  A power of two as the scale means that x / scale is exact, so a
 // value is rounded once, by the conversion, and that a code moves to a greater scale without
-// a further rounding unless it becomes subnormal there.  e4m3 keeps 3 bits behind the
-// leading one over 15 binades, so the scale need not be tight: a factor below two lost at
-// the top costs no precision.
+// a further rounding unless it becomes subnormal there.  The greatest code of a page lies
+// in (224, 448] and the least normal one is 2^-6: values down to between 2^-13.8 and 2^-14.8
+// of the page's greatest keep 3 bits behind the leading one (off by at most 2^-4 of themselves),
+// smaller ones are off by at most 2^-10 * scale.  Against a scale that takes the greatest to 448 itself
+// a power of two costs nothing above and at most one binade there.
 #pragma once
 #include "common.cuh"
 

@@ -17,6 +17,8 @@
 // slice reach, and few others do (of 64 groups and top 20 some 4 more).  The pieces of the threads
 // that may reach it are read once more (from L2) and what does is ranked; the cluster's first CTA
 // merges the slices' lists.
+//
+// Logits are 32-bit, as the decoder's head makes them, or bfloat16, for callers that hold their own so.
 #include "common.cuh"
 
 namespace {
