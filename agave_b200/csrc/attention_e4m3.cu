@@ -82,11 +82,6 @@ struct Tile {
     static constexpr int PART = AE_HEADS * DIM + 2 * AE_HEADS;
 };
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 // 2^(d + e) for d <= 0 and a whole number e as two factors, neither of which leaves the range where their
 // product with something does not; d = -inf: 0.
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((unsigned)(max(e, -126) + 127) << 23); }

@@ -83,12 +83,6 @@ struct AtArgs {
     float cap, cap_in;             // cap_in = 2 log2(e) * scale / cap
 };
 
-// 2^x by the hardware approximation (relative error about 2^-22; -inf gives 0).
-__device__ __forceinline__ float ex2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 // Sum of the lengths before sequence b, each rounded up to a multiple of 64.
 __device__ __forceinline__ int padded_start(const int* cu, int b) {
@@ -436,7 +430,7 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q,
                     // (before the bounds: a capped -infinity is -cap)
 #pragma unroll
                     for (int c = 0; c < 64; ++c) {
-                        const float e = ex2_fast(__uint_as_float(sr[c >> 4][c & 15]) * a.cap_in);
+                        const float e = ex2(__uint_as_float(sr[c >> 4][c & 15]) * a.cap_in);
                         sr[c >> 4][c & 15] =
                             __float_as_uint(fmaf(__fdividef(2.0f, 1.0f + e), -a.cap, a.cap));
                     }
@@ -512,10 +506,10 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q,
                 uint32_t pk[2][16];
 #pragma unroll
                 for (int c = 0; c < 64; c += 4) {
-                    const float p0 = ex2_fast(fmaf(sv[c], a.scale_log2e, neg_m));
-                    const float p1 = ex2_fast(fmaf(sv[c + 1], a.scale_log2e, neg_m));
-                    const float p2 = ex2_fast(fmaf(sv[c + 2], a.scale_log2e, neg_m));
-                    const float p3 = ex2_fast(fmaf(sv[c + 3], a.scale_log2e, neg_m));
+                    const float p0 = ex2(fmaf(sv[c], a.scale_log2e, neg_m));
+                    const float p1 = ex2(fmaf(sv[c + 1], a.scale_log2e, neg_m));
+                    const float p2 = ex2(fmaf(sv[c + 2], a.scale_log2e, neg_m));
+                    const float p3 = ex2(fmaf(sv[c + 3], a.scale_log2e, neg_m));
                     ps[0] += p0, ps[1] += p1, ps[2] += p2, ps[3] += p3;
                     const __nv_bfloat162 t0 = __floats2bfloat162_rn(p0, p1);
                     const __nv_bfloat162 t1 = __floats2bfloat162_rn(p2, p3);

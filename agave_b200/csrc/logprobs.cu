@@ -46,16 +46,6 @@ __device__ __forceinline__ float lp_value(u64 key) {
 }
 __device__ __forceinline__ u64 greater(u64 a, u64 b) { return a > b ? a : b; }
 
-__device__ __forceinline__ float lp_ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-    f32x2 d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
 __device__ __forceinline__ float max_nan(float a, float b) {        // NaN if either is
     float y;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
@@ -67,7 +57,7 @@ struct Sums {
     float c, s, t;
     __device__ __forceinline__ void move(float to) {
         // (a reference of -inf has sums of 0, or NaN, which stay that)
-        const float d = fmaxf(c - to, -1e4f), f = lp_ex2(d * LOG2E);
+        const float d = fmaxf(c - to, -1e4f), f = ex2(d * LOG2E);
         t = f * fmaf(d, s, t);
         s *= f;
         c = to;
@@ -268,7 +258,7 @@ __global__ void __launch_bounds__(LP_THREADS, 1024 / LP_THREADS) logprobs_kernel
                         d = pack2(max_nan(y0, -150.f), max_nan(y1, -150.f));
                     }
                     unpack2(mul2(d, log2e), y0, y1);
-                    const f32x2 p = pack2(lp_ex2(y0), lp_ex2(y1));
+                    const f32x2 p = pack2(ex2(y0), ex2(y1));
                     s = add2(s, p);
                     w = fma2(p, d, w);
                 }
@@ -334,7 +324,7 @@ __global__ void __launch_bounds__(LP_THREADS, 1024 / LP_THREADS) logprobs_kernel
             m = xe;
             sum.move(m);
         }
-        const float d = max_nan(xe - (sum.c == -INFINITY ? 0.f : sum.c), -150.f), p = lp_ex2(d * LOG2E);
+        const float d = max_nan(xe - (sum.c == -INFINITY ? 0.f : sum.c), -150.f), p = ex2(d * LOG2E);
         sum.s += p;
         sum.t = fmaf(p, d, sum.t);
         ahead += xe > xt || (xe == xt && edge < tok);

@@ -29,12 +29,6 @@ namespace {
 __device__ __forceinline__ float silu_f(float t) { return t / (1.0f + expf(-t)); }
 __device__ __forceinline__ float softplus_f(float t) { return t > 20.0f ? t : log1pf(expf(t)); }
 
-// 2^x by the hardware approximation (relative error about 2^-22; below 2^-126 it gives 0).
-__device__ __forceinline__ float ex2_ftz(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 struct StepArgs {
     float* state;              // [n_slots, stride]
@@ -367,7 +361,7 @@ selective_scan_kernel(SelectiveArgs a, RowIn<float> in, StepArgs st, T* __restri
                 float acc = 0.f;
 #pragma unroll
                 for (int s = 0; s < NS; ++s) {
-                    S[s] = fmaf(d.y, B[s], ex2_ftz(d.x * a2[s]) * S[s]);
+                    S[s] = fmaf(d.y, B[s], ex2(d.x * a2[s]) * S[s]);
                     if (PASS != 1) acc = fmaf(S[s], Cv[s], acc);
                 }
                 y[q] = acc;
@@ -436,7 +430,7 @@ segment_begins_kernel(SelectiveArgs a, StepArgs st, Segments sg) {
     const size_t step = (size_t)a.inner * a.N;
 #pragma unroll 4
     for (int s = 0; s < n - 1; ++s) {
-        const float own = at[s * step], d = ex2_ftz(sum[(size_t)s * a.inner] * a2);
+        const float own = at[s * step], d = ex2(sum[(size_t)s * a.inner] * a2);
         at[s * step] = run;
         run = fmaf(d, run, own);
     }
