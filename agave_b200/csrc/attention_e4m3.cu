@@ -6,7 +6,7 @@
 // What bounds it is reading each key and value once, hd + hdv bytes a position and kv head.  The
 // pages of all sequences, 64 positions each, lie on one line, which is cut into equal stretches
 // whatever the sequences' lengths are; a CTA takes a stretch for one kv head and up to 8 of its query heads,
-// and where that begins or ends inside a sequence it leaves a partial result (sum, maximum,
+// and where that begins or ends inside a sequence it leaves a partial result (output, maximum,
 // normaliser), which a second kernel joins.  The stretches follow from the positions on the device,
 // so a recorded launch serves every length.  The CTAs of a stretch, a head each, lie beside each
 // other on the grid and go through it together: a head's 64 to 256 bytes of a position are a part
